@@ -38,7 +38,7 @@
 extern "C" {
 #endif
 
-#define B200Q_VERSION 2
+#define B200Q_VERSION 3
 
 /* ---- error codes ------------------------------------------------------- */
 enum {
@@ -455,6 +455,83 @@ int b200q_tp_reduce_rmsnorm_quant(void* const* peer_partials, void* const* peer_
 int b200q_w8a8_gemm_noalloc(const int8_t* xq, const float* a_scales, const int8_t* qweight,
                             const float* w_scales, const void* bias, void* y, int M, int N,
                             int K, int out_dtype, void* stream);
+
+/* ---- attention over a paged key-value cache ----------------------------------------------
+ *
+ * What stands between the qkv projection and the output projection of a decoder layer
+ * (nanovllm/layers/attention.py:59-89 in the reference, which calls libraries for it):
+ *
+ *   o[i,h] = T( sum_j exp(s[i,h,j] - top[i,h]) * v[j,h/G] / sum_j exp(s[i,h,j] - top[i,h]) )
+ *   s[i,h,j] = scale * (q[i,h] . k[j,h/G]),  G = heads / kv_heads,  top = max over j
+ *
+ * over the keys j that row i sees.  In a sequence with n queries and m keys (0 <= n, m; the queries
+ * are the last n of m positions) causal attention shows row i the keys j <= i + m - n; without
+ * `causal` every row sees all m.  A row that sees no key gives zeros.  Keys that a row does not see do not
+ * reach it whatever they hold, with one exception: a non-finite value v of a later position of the same sequence
+ * may make the rows up to 383 positions before it non-finite, as zero times infinity does in any matrix product.
+ * Sums and softmax statistics are fp32; the weights exp(s - top) are rounded to T once, as operands of the
+ * second product, and the result once.
+ *
+ * 16-bit elements [page][token][head][dim] at data + page * page_stride + token * token_stride + head *
+ * head_stride (strides in elements, multiples of 8, not negative, under 2^39; the innermost dimension is dense, data
+ * 16-byte aligned).
+ */
+typedef struct {
+  void* data;
+  int64_t page, token, head; /* strides */
+} b200q_view;
+
+typedef struct {
+  b200q_view q;          /* [tokens][heads][dim]; the page stride is not used                        */
+  b200q_view k, v;       /* packed: [key_tokens][kv_heads][dim]; paged: [pages][page_size][kv_heads][dim] */
+  void* out;             /* dense [tokens][heads][dim]; rows behind the last sequence are left alone  */
+  const int32_t* cu_q;   /* prefill: [sequences + 1], where each sequence's queries begin             */
+  const int32_t* cu_k;   /* prefill: [sequences + 1], the same of its keys (paged: only the differences count) */
+  const int32_t* lengths;/* decode: [sequences], keys of each sequence, its new token among them       */
+  const int32_t* tables; /* paged: page of positions [i * page_size, (i + 1) * page_size) at tables[b * table_stride + i] */
+  int64_t table_stride;
+  int tokens, key_tokens, sequences;
+  int heads, kv_heads, dim;           /* dim % 8 == 0, dim <= 128; heads / kv_heads <= 128            */
+  int pages, page_size, table_width;  /* page_size 0: packed, else a multiple of 16                   */
+  int max_q, max_k;                   /* bounds of n and m; results do not depend on them              */
+  int causal;
+  int dtype;                          /* B200Q_DTYPE_*                                                 */
+  float scale;
+} b200q_attention;
+
+/*
+ * Sequences of any lengths, packed one after another (n = 0 and m = 0 included).  Decode: one query
+ * per sequence, token b belongs to sequence b, keys and values in pages.  The lengths, tables and
+ * pages are read on the device when the kernel runs, so a captured call follows their contents.
+ * Lengths are cut to what the tables (packed: key_tokens) hold.  A page outside of the cache counts as zeros and sets the
+ * device status word to 0xa01.  workspace: *_workspace_bytes() of the same arguments (0 -> NULL ok);
+ * it holds nothing from one call to the next, and calls that overlap need one each.
+ */
+int b200q_attn_prefill(const b200q_attention* a, void* workspace, size_t workspace_bytes, void* stream);
+int b200q_attn_decode(const b200q_attention* a, void* workspace, size_t workspace_bytes, void* stream);
+size_t b200q_attn_prefill_workspace_bytes(const b200q_attention* a);
+size_t b200q_attn_decode_workspace_bytes(const b200q_attention* a);
+
+/*
+ * Token t's key and value [kv_heads][dim] go to position slots[t] % page_size of page slots[t] / page_size
+ * (nanovllm/layers/attention.py:10-40).  A negative slot is skipped (padding); one outside of the cache is
+ * skipped and sets the device status word to 0xa02.  The slots of a call are distinct: which of two tokens
+ * with one slot stays is not defined.  k, v: page stride not used; the caches as above.
+ */
+int b200q_kv_store(const b200q_view* k, const b200q_view* v, const b200q_view* k_cache,
+                   const b200q_view* v_cache, const int32_t* slots, int tokens, int kv_heads, int dim,
+                   int pages, int page_size, void* stream);
+
+/*
+ * Copies whole pages: page src[i] to page dst[i], in each of `outer` caches (layers, keys and values) that
+ * begin outer_stride bytes apart and whose dense pages of page_bytes begin page_stride bytes apart (all
+ * multiples of 16).  src and dst are HOST arrays, read before the call returns (a captured call keeps its pairs).
+ * A page may be copied to several places; a destination stands once, and no page is source and destination
+ * of one call (B200Q_ERR_BAD_ARGUMENT, as for a page outside of the cache).  No counterpart in the reference.
+ */
+int b200q_kv_copy_pages(void* cache, int64_t outer, int64_t outer_stride, int64_t page_stride,
+                        int64_t page_bytes, int pages, const int32_t* src, const int32_t* dst, int count,
+                        void* stream);
 
 #ifdef __cplusplus
 }

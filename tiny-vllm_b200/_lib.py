@@ -62,7 +62,25 @@ KNOB_NO_MID = 18
 KNOB_NO_REG = 19
 
 # B200Q_VERSION of include/b200q.h this binding was written for
-ABI_VERSION = 2
+ABI_VERSION = 3
+
+
+
+class View(ctypes.Structure):
+    """``b200q_view``: 16-bit elements ``[page][token][head][dim]``, strides in elements."""
+    _fields_ = [("data", ctypes.c_void_p), ("page", ctypes.c_int64), ("token", ctypes.c_int64),
+                ("head", ctypes.c_int64)]
+
+
+class Attention(ctypes.Structure):
+    """``b200q_attention``: the arguments of the attention entry points."""
+    _fields_ = ([(n, View) for n in ("q", "k", "v")]
+                + [(n, ctypes.c_void_p) for n in ("out", "cu_q", "cu_k", "lengths", "tables")]
+                + [("table_stride", ctypes.c_int64)]
+                + [(n, ctypes.c_int) for n in ("tokens", "key_tokens", "sequences", "heads", "kv_heads", "dim", "pages",
+                                               "page_size", "table_width", "max_q", "max_k", "causal", "dtype")]
+                + [("scale", ctypes.c_float)])
+
 
 # every symbol include/b200q.h declares: name -> (restype, argtypes)
 _c = ctypes
@@ -127,6 +145,13 @@ SIGNATURES = {
     "b200q_w8a8_gemm_noalloc": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p,
                                            _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_int, _c.c_int,
                                            _c.c_int, _c.c_void_p]),
+    "b200q_attn_prefill": (_c.c_int, [_c.POINTER(Attention), _c.c_void_p, _c.c_size_t, _c.c_void_p]),
+    "b200q_attn_decode": (_c.c_int, [_c.POINTER(Attention), _c.c_void_p, _c.c_size_t, _c.c_void_p]),
+    "b200q_attn_prefill_workspace_bytes": (_c.c_size_t, [_c.POINTER(Attention)]),
+    "b200q_attn_decode_workspace_bytes": (_c.c_size_t, [_c.POINTER(Attention)]),
+    "b200q_kv_store": (_c.c_int, [_c.POINTER(View)] * 4 + [_c.c_void_p] + [_c.c_int] * 5 + [_c.c_void_p]),
+    "b200q_kv_copy_pages": (_c.c_int, [_c.c_void_p] + [_c.c_int64] * 4 + [_c.c_int, _c.c_void_p, _c.c_void_p,
+                                                                         _c.c_int, _c.c_void_p]),
 }
 
 _lock = threading.Lock()

@@ -81,9 +81,7 @@ inline c10::SmallVector<int64_t, 5> out_shape(const at::Tensor& x, int64_t N) {
   return shape;
 }
 
-PyObject* fail(int rc, const char* where, int64_t M, int64_t N, int64_t K) {
-  const std::string detail =
-      "M=" + std::to_string(M) + " N=" + std::to_string(N) + " K=" + std::to_string(K);
+PyObject* fail(int rc, const char* where, const std::string& detail) {
   if (g_on_error != nullptr) {
     PyObject* r = PyObject_CallFunction(g_on_error, "iss", rc, where, detail.c_str());
     if (r == nullptr) return nullptr;
@@ -91,6 +89,10 @@ PyObject* fail(int rc, const char* where, int64_t M, int64_t N, int64_t K) {
   }
   PyErr_Format(PyExc_RuntimeError, "%s: error %d [%s]", where, rc, detail.c_str());
   return nullptr;
+}
+
+PyObject* fail(int rc, const char* where, int64_t M, int64_t N, int64_t K) {
+  return fail(rc, where, "M=" + std::to_string(M) + " N=" + std::to_string(N) + " K=" + std::to_string(K));
 }
 
 // ------------------------------------------------------------------------- workspace
@@ -414,6 +416,204 @@ PyObject* silu_mul_quant(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------- attention and its cache
+// [rows, heads, dim] or [pages, page size, heads, dim] of 16-bit elements as the library reads it
+bool view_of(const at::Tensor& t, b200q_view* out) {
+  const int64_t n = t.dim();
+  if ((t.size(n - 1) > 1 && t.stride(n - 1) != 1) || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0) return false;
+  out->data = t.data_ptr();
+  for (int64_t i = 0; i + 1 < n; ++i)
+    if (t.size(i) > 1 && t.stride(i) <= 0) return false;
+  out->head = t.size(n - 2) > 1 ? t.stride(n - 2) : 0;      // the stride of a dimension of size one says nothing
+  out->token = t.size(n - 3) > 1 ? t.stride(n - 3) : 0;
+  out->page = n > 3 && t.size(n - 4) > 1 ? t.stride(n - 4) : 0;
+  return out->head % 8 == 0 && out->token % 8 == 0 && out->page % 8 == 0;
+}
+// an int32 tensor on `device`, dense in its last dimension
+inline bool ints(const at::Tensor* t, int64_t dim, const at::Device& device) {
+  return t != nullptr && t->scalar_type() == at::kInt && t->device() == device && t->dim() == dim &&
+         (t->size(dim - 1) <= 1 || t->stride(dim - 1) == 1);
+}
+
+// attention(q, k, v, cu_q | None, cu_k | None, lengths | None, tables | None, max_q, max_k, scale, causal, out | None)
+//   -> out; decode where lengths are given
+PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  B200Q_NEEDS(12)
+  const at::Tensor *q = tensor_of(args[0]), *k = tensor_of(args[1]), *v = tensor_of(args[2]);
+  if (q == nullptr || !q->is_cuda() || q->dim() != 3 || q->numel() == 0 || k == nullptr || v == nullptr) Py_RETURN_NONE;
+  const at::ScalarType type = q->scalar_type();
+  const at::Device device = q->device();
+  b200q_attention a{};
+  a.dtype = dtype_id(type);
+  const bool decode = args[5] != Py_None, paged = args[6] != Py_None;
+  if (a.dtype < 0 || k->scalar_type() != type || v->scalar_type() != type || k->device() != device ||
+      v->device() != device || k->dim() != (paged ? 4 : 3) || k->sizes() != v->sizes() || q->size(2) != k->size(-1) ||
+      (decode && !paged))
+    Py_RETURN_NONE;
+  for (const at::Tensor* t : {q, k})
+    for (int64_t size : t->sizes())
+      if (!fits_int(size)) Py_RETURN_NONE;
+  if (!view_of(*q, &a.q)) Py_RETURN_NONE;
+  if (k->numel() == 0) {      // no sequence has keys: nothing is read
+    if (paged) Py_RETURN_NONE;
+    a.k = a.v = a.q;
+  } else if (!view_of(*k, &a.k) || !view_of(*v, &a.v)) {
+    Py_RETURN_NONE;
+  }
+  a.tokens = static_cast<int>(q->size(0));
+  a.heads = static_cast<int>(q->size(1));
+  a.dim = static_cast<int>(q->size(2));
+  a.kv_heads = static_cast<int>(k->size(-2));
+  if (decode) {
+    const at::Tensor* lengths = tensor_of(args[5]);
+    if (!ints(lengths, 1, device) || lengths->size(0) != a.tokens) Py_RETURN_NONE;
+    a.lengths = static_cast<const int32_t*>(lengths->data_ptr());
+    a.sequences = a.tokens;
+  } else {
+    const at::Tensor *cu_q = tensor_of(args[3]), *cu_k = tensor_of(args[4]);
+    if (!ints(cu_q, 1, device) || !ints(cu_k, 1, device) || cu_q->size(0) < 2 || cu_q->size(0) != cu_k->size(0) ||
+        !fits_int(cu_q->size(0)))
+      Py_RETURN_NONE;
+    a.cu_q = static_cast<const int32_t*>(cu_q->data_ptr());
+    a.cu_k = static_cast<const int32_t*>(cu_k->data_ptr());
+    a.sequences = static_cast<int>(cu_q->size(0) - 1);
+  }
+  if (paged) {
+    const at::Tensor* tables = tensor_of(args[6]);
+    if (!ints(tables, 2, device) || tables->size(0) != a.sequences || tables->size(1) == 0 || !fits_int(tables->size(1)))
+      Py_RETURN_NONE;
+    a.tables = static_cast<const int32_t*>(tables->data_ptr());
+    a.table_stride = tables->size(0) > 1 ? tables->stride(0) : 0;
+    a.table_width = static_cast<int>(tables->size(1));
+    a.pages = static_cast<int>(k->size(0));
+    a.page_size = static_cast<int>(k->size(1));
+  } else {
+    a.key_tokens = static_cast<int>(k->size(0));
+  }
+  const long max_q = PyLong_AsLong(args[7]), max_k = PyLong_AsLong(args[8]);
+  const double scale = PyFloat_AsDouble(args[9]);
+  a.causal = PyObject_IsTrue(args[10]);
+  if (PyErr_Occurred()) return nullptr;
+  if (!fits_int(max_q) || !fits_int(max_k)) Py_RETURN_NONE;
+  a.max_q = static_cast<int>(max_q);
+  a.max_k = static_cast<int>(max_k);
+  a.scale = static_cast<float>(scale);
+  c10::cuda::CUDAGuard guard(device);
+  at::Tensor out;
+  if (args[11] == Py_None) {
+    out = empty_on(q->sizes(), type, device);
+  } else {
+    const at::Tensor* given = tensor_of(args[11]);
+    if (!dense(given, type, device) || given->sizes() != q->sizes()) Py_RETURN_NONE;
+    out = *given;
+  }
+  a.out = out.data_ptr();
+  // Partial results of this call alone: calls on several streams, and captured graphs, each have their own.
+  at::Tensor ws;
+  const size_t bytes = decode ? b200q_attn_decode_workspace_bytes(&a) : b200q_attn_prefill_workspace_bytes(&a);
+  if (bytes > 0) ws = empty_on({static_cast<int64_t>(bytes)}, at::kByte, device);
+  const int rc = unlocked([&] {
+    return (decode ? b200q_attn_decode : b200q_attn_prefill)(&a, bytes > 0 ? ws.data_ptr() : nullptr, bytes,
+                                                             stream_of(device));
+  });
+  if (rc != B200Q_OK)
+    return fail(rc, decode ? "b200q_attn_decode" : "b200q_attn_prefill",
+                "tokens=" + std::to_string(a.tokens) + " heads=" + std::to_string(a.heads) + "/" +
+                    std::to_string(a.kv_heads) + " dim=" + std::to_string(a.dim) +
+                    " page_size=" + std::to_string(a.page_size));
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// kv_store(k, v, k_cache, v_cache, slots) -> True, or None
+PyObject* kv_store(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  B200Q_NEEDS(5)
+  const at::Tensor* t[4];
+  b200q_view view[4];
+  for (int i = 0; i < 4; ++i) t[i] = tensor_of(args[i]);
+  if (t[0] == nullptr || !t[0]->is_cuda() || t[0]->numel() == 0 || dtype_id(t[0]->scalar_type()) < 0) Py_RETURN_NONE;
+  const at::Device device = t[0]->device();
+  for (int i = 0; i < 4; ++i)
+    if (t[i] == nullptr || t[i]->device() != device || t[i]->scalar_type() != t[0]->scalar_type() ||
+        t[i]->dim() != (i < 2 ? 3 : 4) || t[i]->sizes() != t[i & 2]->sizes() || t[i]->numel() == 0 ||
+        !view_of(*t[i], &view[i]))
+      Py_RETURN_NONE;
+  const at::Tensor* slots = tensor_of(args[4]);
+  const int64_t tokens = t[0]->size(0), heads = t[0]->size(1), dim = t[0]->size(2);
+  if (!ints(slots, 1, device) || slots->size(0) != tokens || t[2]->size(2) != heads || t[2]->size(3) != dim) Py_RETURN_NONE;
+  for (int64_t size : {tokens, heads, dim, t[2]->size(0), t[2]->size(1)})
+    if (!fits_int(size)) Py_RETURN_NONE;
+  c10::cuda::CUDAGuard guard(device);
+  const int rc = unlocked([&] {
+    return b200q_kv_store(&view[0], &view[1], &view[2], &view[3], static_cast<const int32_t*>(slots->data_ptr()),
+                          static_cast<int>(tokens), static_cast<int>(heads), static_cast<int>(dim),
+                          static_cast<int>(t[2]->size(0)), static_cast<int>(t[2]->size(1)), stream_of(device));
+  });
+  if (rc != B200Q_OK)
+    return fail(rc, "b200q_kv_store", "tokens=" + std::to_string(tokens) + " heads=" + std::to_string(heads) +
+                                          " dim=" + std::to_string(dim));
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// a sequence of ints -> int32; false (and no error set) where one is none or does not fit
+bool int32s(PyObject* o, std::vector<int32_t>* out) {
+  PyObject* fast = PySequence_Fast(o, "");
+  if (fast == nullptr) {
+    PyErr_Clear();
+    return false;
+  }
+  bool ok = true;
+  out->reserve(PySequence_Fast_GET_SIZE(fast));
+  for (Py_ssize_t i = 0; ok && i < PySequence_Fast_GET_SIZE(fast); ++i) {
+    const long long x = PyLong_AsLongLong(PySequence_Fast_GET_ITEM(fast, i));
+    ok = !PyErr_Occurred() && x >= INT_MIN && x <= INT_MAX;
+    out->push_back(static_cast<int32_t>(x));
+  }
+  PyErr_Clear();
+  Py_DECREF(fast);
+  return ok;
+}
+
+// copy_pages(cache [..., pages, page size, heads, dim], src, dst) -> True, or None
+PyObject* copy_pages(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  B200Q_NEEDS(3)
+  const at::Tensor* cache = tensor_of(args[0]);
+  if (cache == nullptr || !cache->is_cuda() || cache->dim() < 4 || cache->numel() == 0) Py_RETURN_NONE;
+  const int64_t n = cache->dim();
+  // dense pages, and one stride over the leading dimensions
+  int64_t inner = 1, outer = 1, outer_stride = 0;
+  for (int64_t i = n - 1; i > n - 4; --i) {
+    if (cache->size(i) > 1 && cache->stride(i) != inner) Py_RETURN_NONE;
+    inner *= cache->size(i);
+  }
+  for (int64_t i = n - 5; i >= 0; --i) {
+    if (cache->size(i) == 1) continue;
+    if (outer == 1) outer_stride = cache->stride(i);
+    if (cache->stride(i) != outer_stride * outer) Py_RETURN_NONE;
+    outer *= cache->size(i);
+  }
+  std::vector<int32_t> src, dst;
+  if (!int32s(args[1], &src) || !int32s(args[2], &dst) || src.size() != dst.size() || src.empty() ||
+      !fits_int(cache->size(n - 4)) || !fits_int(static_cast<int64_t>(src.size())))
+    Py_RETURN_NONE;
+  const int64_t bytes = cache->element_size(), page_stride = cache->size(n - 4) > 1 ? cache->stride(n - 4) : inner;
+  c10::cuda::CUDAGuard guard(cache->device());
+  const int rc = unlocked([&] {
+    return b200q_kv_copy_pages(cache->data_ptr(), outer, outer_stride * bytes, page_stride * bytes, inner * bytes,
+                               static_cast<int>(cache->size(n - 4)), src.data(), dst.data(),
+                               static_cast<int>(src.size()), stream_of(cache->device()));
+  });
+  if (rc != B200Q_OK)
+    return fail(rc, "b200q_kv_copy_pages", "pages=" + std::to_string(cache->size(n - 4)) +
+                                               " page_bytes=" + std::to_string(inner * bytes));
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
 // reserve(bytes, device index | -1): raises the floor of the workspace size; with a device the
 // buffer is allocated now
 PyObject* reserve(PyObject*, PyObject* args) {
@@ -449,6 +649,9 @@ PyMethodDef g_methods[] = {B200Q_FAST(w8a16),
                            B200Q_FAST(quantize),
                            B200Q_FAST(rmsnorm_quant),
                            B200Q_FAST(silu_mul_quant),
+                           B200Q_FAST(attention),
+                           B200Q_FAST(kv_store),
+                           B200Q_FAST(copy_pages),
                            {"reserve", reserve, METH_VARARGS, nullptr},
                            {"set_error_handler", set_error_handler, METH_O, nullptr},
                            {nullptr, nullptr, 0, nullptr}};

@@ -1,6 +1,8 @@
-"""Layers on the quantized-linear path (reference: ``nanovllm/layers/linear.py``)."""
+"""Layers of the decoder: quantized linears (reference: ``nanovllm/layers/linear.py``) and attention
+(``nanovllm/layers/attention.py``)."""
+from .attention import Attention
 from .linear import (ColumnParallelLinear, LinearBase, MergedColumnParallelLinear,
                      QKVParallelLinear, ReplicatedLinear, RowParallelLinear)
 
-__all__ = ["LinearBase", "ReplicatedLinear", "ColumnParallelLinear",
+__all__ = ["Attention", "LinearBase", "ReplicatedLinear", "ColumnParallelLinear",
            "MergedColumnParallelLinear", "QKVParallelLinear", "RowParallelLinear"]
