@@ -114,13 +114,16 @@ int check(const b200q_attention* a, bool decode) {
   return B200Q_OK;
 }
 
-int run(const b200q_attention* a, bool decode, void* stream) {
+int run(const b200q_attention* a, bool decode, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check(a, decode)) return rc;
+  const size_t need = decode ? attn_decode_workspace(*a) : 0;
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return B200Q_ERR_WORKSPACE;
+  if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return B200Q_ERR_MISALIGNED;
   int* status = device_status_ptr();
   if (status == nullptr) return B200Q_ERR_LAUNCH;
   if (device_cc_major() != 10) return B200Q_ERR_UNSUPPORTED_ARCH;
+  if (decode) return launch_attn_decode(*a, workspace, status, static_cast<cudaStream_t>(stream));
   b200q_attention c = *a;
-  if (decode) c.cu_q = nullptr;
   auto kernel = c.dtype == B200Q_DTYPE_BF16 ? attn_rows_kernel<__nv_bfloat16> : attn_rows_kernel<__half>;
   cudaError_t e = launch_overlapped(DEFAULT_SPLIT, kernel, dim3(c.tokens, (c.heads + 3) / 4), dim3(128), 0,
                                     static_cast<cudaStream_t>(stream), c, status);
@@ -139,9 +142,17 @@ using namespace b200q;
 
 extern "C" {
 
-int b200q_attn_prefill(const b200q_attention* a, void*, size_t, void* stream) { return run(a, false, stream); }
-int b200q_attn_decode(const b200q_attention* a, void*, size_t, void* stream) { return run(a, true, stream); }
-size_t b200q_attn_prefill_workspace_bytes(const b200q_attention*) { return 0; }
-size_t b200q_attn_decode_workspace_bytes(const b200q_attention*) { return 0; }
+int b200q_attn_prefill(const b200q_attention* a, void* workspace, size_t workspace_bytes, void* stream) {
+  return run(a, false, workspace, workspace_bytes, stream);
+}
+
+int b200q_attn_decode(const b200q_attention* a, void* workspace, size_t workspace_bytes, void* stream) {
+  return run(a, true, workspace, workspace_bytes, stream);
+}
+
+size_t b200q_attn_prefill_workspace_bytes(const b200q_attention* a) { return check(a, false) == B200Q_OK ? 0 : 0; }
+size_t b200q_attn_decode_workspace_bytes(const b200q_attention* a) {
+  return check(a, true) == B200Q_OK ? attn_decode_workspace(*a) : 0;
+}
 
 }  // extern "C"

@@ -28,6 +28,7 @@
 #include <unordered_map>
 #include <vector>
 
+#include "attn.h"
 #include "common.h"
 #include "ptx_sm100.cuh"
 #include "w8a8_device.cuh"
@@ -417,6 +418,29 @@ bool make_tensor_map(const void* base, uint64_t rows, uint64_t row_bytes, uint32
                   strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    note_cuda_error(cudaErrorInvalidValue);
+    return false;
+  }
+  g_maps_encoded.fetch_add(1, std::memory_order_relaxed);
+  return true;
+}
+
+bool make_tensor_map_16(const void* base, int dims, const uint64_t* size, const int64_t* stride, const uint32_t* box,
+                        CUtensorMap* out) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return false;
+  cuuint64_t bytes[4], extent[5];
+  cuuint32_t b[5], estr[5] = {1, 1, 1, 1, 1};
+  for (int i = 0; i < dims; ++i) {
+    extent[i] = size[i];
+    b[i] = box[i];
+    if (i > 0) bytes[i - 1] = static_cast<cuuint64_t>(stride[i - 1]) * 2;
+  }
+  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, dims, const_cast<void*>(base), extent, bytes, b, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  size[0] > 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     note_cuda_error(cudaErrorInvalidValue);
     return false;
