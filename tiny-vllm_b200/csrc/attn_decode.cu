@@ -61,7 +61,8 @@ struct DecodeParams {
 };
 
 __device__ __forceinline__ int clipped(int n, const DecodeParams& p) {
-  return static_cast<int>(min(static_cast<int64_t>(max(n, 0)), static_cast<int64_t>(p.table_width) * p.page_size));
+  return static_cast<int>(min(static_cast<int64_t>(min(max(n, 0), INT_MAX - kTile)),
+                              static_cast<int64_t>(p.table_width) * p.page_size));
 }
 __device__ __forceinline__ int tiles_of(int length) { return max(1, (length + kTile - 1) / kTile); }
 

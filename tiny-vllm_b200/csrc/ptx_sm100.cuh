@@ -228,6 +228,14 @@ __device__ __forceinline__ uint64_t umma_desc_k_sw128(uint32_t smem_addr) {
   return d;
 }
 
+// The same for an operand stored the other way round, as rows of K with 64 16-bit elements of M or N each (128 bytes, 128-byte
+// swizzle): groups of eight rows of K are 1024 bytes apart, the next 64 elements of M or N `block_bytes` further.  Advancing
+// along K by 16 rows adds 2048 >> 4 to the low word.
+__device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t smem_addr, uint32_t block_bytes) {
+  return umma_desc_k_sw128(smem_addr) - (static_cast<uint64_t>(1u) << 16) +
+         (static_cast<uint64_t>(block_bytes >> 4) << 16);
+}
+
 // Instruction descriptor, dense, both operands K-major, D is M x N.
 //   c_format: 1 = fp32, 2 = int32; ab_format: kind::i8 -> 1 = signed int8;
 //   kind::f16 -> 0 = fp16, 1 = bf16.
@@ -236,6 +244,7 @@ __device__ __host__ __forceinline__ uint32_t umma_idesc(uint32_t c_format, uint3
   return (c_format << 4) | (ab_format << 7) | (ab_format << 10) | ((n >> 3) << 17) |
          ((m >> 4) << 24);
 }
+constexpr uint32_t kIdescMnMajorB = 1u << 16;   // B is stored as rows of K
 
 // Reads 32 consecutive 32-bit columns of this thread's TMEM lane.
 __device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&v)[32]) {
@@ -450,6 +459,17 @@ __device__ __forceinline__ void bulk_wait_group() {
 // Named barrier among a subset of the CTA's warps.
 __device__ __forceinline__ void named_bar_sync(uint32_t id, uint32_t nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
+}
+
+// Registers of the warps of a warpgroup (all of its warps take part): more for some, from what others give up.  The sum over
+// the CTA must stay within what it was launched with.
+template <int N>
+__device__ __forceinline__ void raise_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void lower_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 // ---- programmatic dependent launch.  A kernel launched with the programmatic-serialization
