@@ -496,7 +496,7 @@ typedef struct {
   int max_q, max_k;                   /* bounds of n and m; results do not depend on them              */
   int causal;
   int dtype;                          /* B200Q_DTYPE_*                                                 */
-  float scale;
+  float scale;                        /* positive, under 1e38 */
 } b200q_attention;
 
 /*

@@ -1,8 +1,6 @@
 // Attention: the C entry points and what they refuse.
 #include <cuda_runtime.h>
 
-#include <cmath>
-
 #include "attn.h"
 #include "common.h"
 
@@ -16,7 +14,7 @@ int check(const b200q_attention* a, bool decode) {
       (paged && a->tables == nullptr))
     return B200Q_ERR_NULL_POINTER;
   if (a->dtype != B200Q_DTYPE_F16 && a->dtype != B200Q_DTYPE_BF16) return B200Q_ERR_BAD_ARGUMENT;
-  if (!std::isfinite(a->scale) || a->scale < 0) return B200Q_ERR_BAD_ARGUMENT;
+  if (!(a->scale > 0) || !(a->scale < 1e38f)) return B200Q_ERR_BAD_ARGUMENT;
   if (a->tokens <= 0 || a->sequences <= 0 || a->heads <= 0 || a->kv_heads <= 0 || a->dim <= 0 || a->max_q < 0 || a->max_k < 0)
     return B200Q_ERR_BAD_SHAPE;
   if (decode && (!paged || a->tokens != a->sequences)) return B200Q_ERR_BAD_SHAPE;

@@ -84,17 +84,17 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
   uint8_t* ring = smem + 2 * kTileBytes;
   uint8_t* ctrl = ring + kStages * kTileBytes;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(ctrl);   // [stages] a K or V tile is there
-  uint64_t* empty_bar = full_bar + kStages;                 // [stages] products that read it are done
-  uint64_t* s_bar = empty_bar + kStages;                    // [2] scores of a tile are there
-  uint64_t* p_bar = s_bar + 2;                              // [2] its weights are
-  uint64_t* o_bar = p_bar + 2;                              // [2] a product into O is done
-  uint64_t* q_bar = o_bar + 2;
+  uint64_t* free_bar = full_bar + kStages;                  // [4], in turn: products up to a step are done
+  uint64_t* s_bar = free_bar + 4;                           // [2] scores of a tile are there
+  uint64_t* p_bar = s_bar + 2;                              // [2][2] its weights are, of half of the keys
+  uint64_t* o_bar = p_bar + 4;                              // all products are done
+  uint64_t* q_bar = o_bar + 1;
   uint64_t* tail_bar = q_bar + 1;                           // the last V tile, before its end is zeroed
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail_bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* scan = reinterpret_cast<int*>(tmem_slot + 2);        // [warps]
   Item* s_item = reinterpret_cast<Item*>(scan + kThreads / 32);
-  static_assert(8 * (2 * kStages + 8) + 8 + kThreads / 8 + sizeof(Item) <= kCtrlBytes, "control words");
+  static_assert(8 * (kStages + 13) + 8 + kThreads / 8 + sizeof(Item) <= kCtrlBytes, "control words");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t smem_base = ptx::smem_u32(smem), ring_base = smem_base + 2 * kTileBytes;
@@ -103,15 +103,14 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     return;
   }
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
-      ptx::mbar_init(ptx::smem_u32(full_bar + s), 1);
-      ptx::mbar_init(ptx::smem_u32(empty_bar + s), 1);
-    }
+    for (int s = 0; s < kStages; ++s) ptx::mbar_init(ptx::smem_u32(full_bar + s), 1);
+    for (int e = 0; e < 4; ++e) ptx::mbar_init(ptx::smem_u32(free_bar + e), 1);
     for (int t = 0; t < 2; ++t) {
       ptx::mbar_init(ptx::smem_u32(s_bar + t), 1);
-      ptx::mbar_init(ptx::smem_u32(p_bar + t), 4);
-      ptx::mbar_init(ptx::smem_u32(o_bar + t), 1);
+      ptx::mbar_init(ptx::smem_u32(p_bar + 2 * t), 4);
+      ptx::mbar_init(ptx::smem_u32(p_bar + 2 * t + 1), 4);
     }
+    ptx::mbar_init(ptx::smem_u32(o_bar), 1);
     ptx::mbar_init(ptx::smem_u32(q_bar), 1);
     ptx::mbar_init(ptx::smem_u32(tail_bar), 1);
     *abort_flag = 0;
@@ -171,9 +170,10 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     __syncthreads();
   }
   const Item it = *s_item;
-  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t tmem_base = *tmem_slot;      // all columns: 0, which the products' constants rely on
+  if (tmem_base != 0 && threadIdx.x == 0) atomicCAS(p.status, 0, 0x200);
 
-  if (it.b >= 0) {
+  if (it.b >= 0 && tmem_base == 0) {
     // Keys that query i sees: [0, seen(i)).
     const auto seen = [&](int i) { return max(0, p.causal ? min(it.m, i + 1 + it.m - it.n) : it.m); };
     int tiles[2], steps = 0;      // of keys
@@ -201,16 +201,13 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       __syncwarp();
       const int boxes = kRows / p.box_rows;
       const int32_t* table = p.page_size > 0 ? p.tables + it.b * p.table_stride : nullptr;
-      int stage = 0;
+      int stage = 0, freed = 0, page = 0;
       uint32_t phase = 0;
-      int page = 0;
       for (int s = 0; s < steps; ++s) {
         const int begin = (steps - 1 - s) * kRows;
-        const int held = p.page_size > 0 ? min(boxes, (it.m - begin + p.box_rows - 1) / p.box_rows) : 1;
-        int at = it.key0 + begin;
+        int at = it.key0 + begin, held = 1, mine = 0;
         if (p.page_size > 0) {
           // pages of the next 32 boxes at a time, from the last key backwards
-          const int box = s * boxes + (boxes - 1 - lane);           // lane < boxes
           if (s * boxes % 32 == 0) {
             const int64_t pos = static_cast<int64_t>(steps) * kRows - static_cast<int64_t>(s * boxes + lane + 1) * p.box_rows;
             page = 0;
@@ -222,38 +219,27 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
               }
             }
           }
+          mine = __shfl_sync(~0u, page, (s * boxes + boxes - 1 - lane) & 31);
           at = (begin + lane * p.box_rows) % p.page_size;
-          const int mine = __shfl_sync(~0u, page, box & 31);
+          held = min(boxes, (it.m - begin + p.box_rows - 1) / p.box_rows);
+        }
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if (alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(empty_bar + stage), phase ^ 1u, abort_flag));
-            const uint32_t bar = ptx::smem_u32(x == 1 && s == 0 && tail ? tail_bar : full_bar + stage);
-            if (lane == 0 && alive) ptx::mbar_arrive_expect_tx(bar, held * p.box_rows * D * 2);
-            __syncwarp();
-            if (lane < held && alive)
-              for (int h = 0; h < kHalves; ++h)
-                ptx::tma_load_4d(ring_base + stage * kTileBytes + h * kHalfBytes + lane * p.box_rows * 128,
-                                 x == 0 ? &tmap_k : &tmap_v, bar, h * 64, kv, at, mine);
-            if (++stage == kStages) {
-              stage = 0;
-              phase ^= 1u;
-            }
-          }
-        } else {
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if (alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(empty_bar + stage), phase ^ 1u, abort_flag));
-            const uint32_t bar = ptx::smem_u32(x == 1 && s == 0 && tail ? tail_bar : full_bar + stage);
-            if (lane == 0 && alive) {
-              ptx::mbar_arrive_expect_tx(bar, kTileBytes);
-              for (int h = 0; h < kHalves; ++h)
-                ptx::tma_load_4d(ring_base + stage * kTileBytes + h * kHalfBytes, x == 0 ? &tmap_k : &tmap_v, bar, h * 64, kv,
-                                 at, 0);
-            }
-            if (++stage == kStages) {
-              stage = 0;
-              phase ^= 1u;
-            }
+        for (int x = 0; x < 2; ++x) {
+          // Tile n = 2 s + x takes the place of tile n - kStages: the first key tile is free with the first signal, and the
+          // values of step e - 1 and the keys of step e with signal e.
+          const int need = (2 * s + x - kStages + 1) >> 1;
+          for (; freed <= need; ++freed)
+            if (alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(free_bar + (freed & 3)), (freed >> 2) & 1, abort_flag));
+          const uint32_t bar = ptx::smem_u32(x == 1 && s == 0 && tail ? tail_bar : full_bar + stage);
+          if (lane == 0 && alive) ptx::mbar_arrive_expect_tx(bar, held * p.box_rows * D * 2);
+          __syncwarp();
+          if (lane < held && alive)
+            for (int h = 0; h < kHalves; ++h)
+              ptx::tma_load_4d(ring_base + stage * kTileBytes + h * kHalfBytes + lane * p.box_rows * 128,
+                               x == 0 ? &tmap_k : &tmap_v, bar, h * 64, kv, at, mine);
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
           }
         }
       }
@@ -265,69 +251,64 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     } else if (warp == 8) {
       ptx::lower_registers<kOtherRegs>();
       // ---------------------------------------------------------------- products
-      if (lane == 0 && steps > 0) {
-        constexpr uint32_t ab = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-        const uint32_t idesc_s = ptx::umma_idesc(1u, ab, kRows, kRows);
-        const uint32_t idesc_o = ptx::umma_idesc(1u, ab, kRows, D) | ptx::kIdescMnMajorB;
-        int stage = 0;
-        uint32_t phase = 0;
-        bool ok = ptx::mbar_wait(ptx::smem_u32(q_bar), 0, abort_flag);
-        const auto scores = [&](int t, int at) {
+      // The whole warp walks and one lane issues.
+      constexpr uint32_t ab = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+      const uint32_t idesc_s = ptx::umma_idesc(1u, ab, kRows, kRows);
+      const uint32_t idesc_o = ptx::umma_idesc(1u, ab, kRows, D) | ptx::kIdescMnMajorB;
+      const uint64_t q_desc = ptx::umma_desc_k_sw128(smem_base), k_desc = ptx::umma_desc_k_sw128(ring_base);
+      const uint64_t v_desc = ptx::umma_desc_mn_sw128(ring_base, kHalfBytes);
+      const bool one = ptx::elect_one();
+      bool ok = true;
+      const auto scores = [&](int t, int at) {
+        const uint64_t q = q_desc + t * (kTileBytes >> 4), keys = k_desc + at * (kTileBytes >> 4);
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t off = (k >> 2) * kHalfBytes + (k & 3) * 32;
-            ptx::umma_f16_ss(tmem_base + t * kRows, ptx::umma_desc_k_sw128(smem_base + t * kTileBytes + off),
-                             ptx::umma_desc_k_sw128(ring_base + at * kTileBytes + off), idesc_s, k > 0);
-          }
-          ptx::umma_commit(ptx::smem_u32(s_bar + t));
-        };
-        if (ok) ok = ptx::mbar_wait(ptx::smem_u32(full_bar), 0, abort_flag);
-        if (ok) {
-          ptx::tc_fence_after_sync();
-          for (int t = 0; t < 2; ++t)
-            if (skip[t] == 0) scores(t, 0);
-          ptx::umma_commit(ptx::smem_u32(empty_bar));
+        for (int k = 0; k < D / 16; ++k) {
+          const int off = ((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4;
+          ptx::umma_f16_ss_by(one && ok, t * kRows, q + off, keys + off, idesc_s, k > 0);
         }
-        stage = 1;
-        for (int s = 0; ok && s < steps; ++s) {
-          const int v_stage = stage, k_stage = stage + 1 == kStages ? 0 : stage + 1;
-          const uint32_t v_phase = phase, k_phase = k_stage == 0 ? phase ^ 1u : phase;
-          const bool more = s + 1 < steps;
-          if (!ptx::mbar_wait(ptx::smem_u32(full_bar + v_stage), v_phase, abort_flag)) {
-            ok = false;
-            break;
-          }
-          for (int t = 0; t < 2; ++t) {
-            if (s >= skip[t]) {
-              if (!ptx::mbar_wait(ptx::smem_u32(p_bar + t), (s - skip[t]) & 1, abort_flag)) {
-                ok = false;
-                break;
-              }
+        ptx::umma_commit_by(one && ok, ptx::smem_u32(s_bar + t));
+      };
+      int stage = 1;
+      uint32_t phase = 0;
+      if (steps > 0)
+        ok = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(q_bar), 0, abort_flag) &&
+                           ptx::mbar_wait(ptx::smem_u32(full_bar), 0, abort_flag));
+      ptx::tc_fence_after_sync();
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        if (tiles[t] > 0 && skip[t] == 0) scores(t, 0);
+      ptx::umma_commit_by(one && ok, ptx::smem_u32(free_bar));
+      for (int s = 0; s < steps; ++s) {
+        const int v_stage = stage, k_stage = stage + 1 == kStages ? 0 : stage + 1;
+        const uint32_t v_phase = phase, k_phase = k_stage == 0 ? phase ^ 1u : phase;
+        const bool more = s + 1 < steps;
+        const uint64_t values = v_desc + v_stage * (kTileBytes >> 4);
+        if (ok)
+          ok = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(full_bar + v_stage), v_phase, abort_flag) &&
+                             (!more || ptx::mbar_wait(ptx::smem_u32(full_bar + k_stage), k_phase, abort_flag)));
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (s >= skip[t]) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              if (ok) ok = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(p_bar + 2 * t + c), (s - skip[t]) & 1, abort_flag));
               ptx::tc_fence_after_sync();
 #pragma unroll
-              for (int k = 0; k < kRows / 16; ++k)
-                ptx::umma_f16_ts(tmem_base + kColO + t * kRows, tmem_base + t * kRows + 8 * k,
-                                 ptx::umma_desc_mn_sw128(ring_base + v_stage * kTileBytes + k * 2048, kHalfBytes), idesc_o,
-                                 s > skip[t] || k > 0);
-              ptx::umma_commit(ptx::smem_u32(o_bar + t));
-            }
-            if (more && t == 0) {
-              if (!ptx::mbar_wait(ptx::smem_u32(full_bar + k_stage), k_phase, abort_flag)) {
-                ok = false;
-                break;
+              for (int i = 0; i < kRows / 32; ++i) {
+                const int k = c * (kRows / 32) + i;
+                ptx::umma_f16_ts_by(one && ok, kColO + t * kRows, t * kRows + 8 * k, values + k * (2048 >> 4), idesc_o,
+                                    s > skip[t] || k > 0);
               }
-              ptx::tc_fence_after_sync();
             }
-            if (more && s + 1 >= skip[t]) scores(t, k_stage);
           }
-          ptx::umma_commit(ptx::smem_u32(empty_bar + v_stage));
-          if (more) ptx::umma_commit(ptx::smem_u32(empty_bar + k_stage));
-          for (int x = 0; x < 2; ++x)
-            if (++stage == kStages) {
-              stage = 0;
-              phase ^= 1u;
-            }
+          if (more && s + 1 >= skip[t]) scores(t, k_stage);
         }
+        ptx::umma_commit_by(one && ok, more ? ptx::smem_u32(free_bar + ((s + 1) & 3)) : ptx::smem_u32(o_bar));
+        for (int x = 0; x < 2; ++x)
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
       }
     } else if (warp >= 8) {
       ptx::lower_registers<kOtherRegs>();
@@ -373,7 +354,11 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         }
         float most[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-        for (int c = 4; c < kRows; ++c) most[c & 3] = fmaxf(most[c & 3], x[c]);
+        for (int c = 4; c + 8 <= kRows; c += 8)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) most[i] = max3(most[i], x[c + 2 * i], x[c + 2 * i + 1]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most[i] = fmaxf(most[i], x[kRows - 4 + i]);
         const float next = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * p.scale_log2;
         if (turn == 0) {
           top = next;
@@ -382,9 +367,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
           const float f = raised == top ? 1.f : exp2_approx(top - raised);
           top = raised;
           sum *= f;
-          alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(o_bar + t), (turn - 1) & 1, abort_flag));
-          if (!alive) break;
-          ptx::tc_fence_after_sync();
+          // (the scores were issued behind the last product into O, so that is done as well)
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {
             uint32_t o[32];
@@ -396,31 +379,40 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
           }
         }
         const float base = top == -INFINITY ? 0.f : top;
-        float part[4] = {0.f, 0.f, 0.f, 0.f};
+        // The exponential unit gives 16 results a cycle for the SM; every fourth pair goes through the multipliers instead.
+        const uint64_t scale2 = pair(p.scale_log2, p.scale_log2), base2 = pair(-base, -base);
+        uint64_t part[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t w[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            const float a = exp2_approx(fmaf(x[64 * c + 2 * i], p.scale_log2, -base));
-            const float b = exp2_approx(fmaf(x[64 * c + 2 * i + 1], p.scale_log2, -base));
-            part[(2 * i) & 3] += a;
-            part[(2 * i + 1) & 3] += b;
-            w[i] = pack16<T>(a, b);
+            const uint64_t arg = fma2(pair(x[64 * c + 2 * i], x[64 * c + 2 * i + 1]), scale2, base2);
+            float2 e;
+            if (i % 4 == 3) {
+              e = exp2_poly(arg);
+            } else {
+              e = unpair(arg);
+              e = make_float2(exp2_approx(e.x), exp2_approx(e.y));
+            }
+            part[i & 1] = add2(part[i & 1], pair(e.x, e.y));
+            w[i] = pack16<T>(e.x, e.y);
           }
           ptx::tmem_st_32x32b_x32(col_s + 32 * c, w);
+          // the product of this half may begin
+          ptx::tmem_st_wait();
+          ptx::tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(p_bar + 2 * t + c));
         }
-        sum += (part[0] + part[1]) + (part[2] + part[3]);
-        ptx::tmem_st_wait();
-        ptx::tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(p_bar + t));
+        const float2 both = unpair(add2(part[0], part[1]));
+        sum += both.x + both.y;
       }
       const int head = kv * p.group + row % p.group;
       uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(p.out) +
                                             (static_cast<int64_t>(it.row0 + query) * p.heads + head) * p.dim);
       const bool any = tiles[t] > 0;
-      if (any && alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(o_bar + t), (tiles[t] - 1) & 1, abort_flag));
+      if (any && alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(o_bar), 0, abort_flag));
       ptx::tc_fence_after_sync();
       const float inv = limit > 0 ? 1.f / sum : 0.f;
 #pragma unroll
