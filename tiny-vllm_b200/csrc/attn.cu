@@ -20,7 +20,7 @@ int check(const b200q_attention* a, bool decode) {
   if (decode && (!paged || a->tokens != a->sequences)) return B200Q_ERR_BAD_SHAPE;
   if (paged ? a->pages <= 0 || a->page_size < 0 || a->table_width <= 0 || a->table_stride < 0 : a->key_tokens < 0)
     return B200Q_ERR_BAD_SHAPE;
-  if (a->heads % a->kv_heads != 0) return B200Q_ERR_BAD_SHAPE;
+  if (a->heads % a->kv_heads != 0 || a->heads > (1 << 15)) return B200Q_ERR_BAD_SHAPE;
   if (a->dim % 8 != 0 || a->dim > 128 || a->heads / a->kv_heads > 128 || a->page_size % 16 != 0)
     return B200Q_ERR_UNSUPPORTED_SHAPE;
   for (const b200q_view* x : {&a->q, &a->k, &a->v})

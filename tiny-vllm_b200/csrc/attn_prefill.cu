@@ -13,10 +13,17 @@
 // O0, O1 (128 x D sums).  Shared memory: both Q tiles and a ring of K and V tiles.
 //   S_t = Q_t K^T    both operands in shared memory
 //   O_t += P_t V      P from tensor memory, V as rows of keys
-// Warps: 0-3 and 4-7 softmax of tile 0 and 1, a row a thread; 8 issues the products; 9 brings Q, K and V; 10 and 11
-// only give their registers up.
 // Keys go from the last tile, where the mask is, to the first.  The running maximum is raised, and O_t rescaled in place, only
 // when a score exceeds it by more than 8 (weights reach 2^8 at most, rounded with the same relative error).
+//
+// Work: an item is two tiles of queries and their keys.  Where there are more items than SMs, or one of them might be long, a
+// small kernel (attn_plan_kernel) lists them first, those with the most keys at the front, and CTAs, one an SM, take one
+// after another; the next item's Q and K arrive, and its first scores are formed, under the last exponentials and the output
+// of the one before.  An item with more than an SM's share of all keys is cut into pieces, which leave fp32 partial
+// results for a third kernel to join in their order: few queries over a long cached prefix then use the whole GPU.
+//
+// Warps: 0-3 and 4-7 softmax of tile 0 and 1, a row a thread; 8 issues the products; 9 brings Q, K and V; 10 fetches
+// items; 11 clears the end of a sequence's last V tile.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -36,17 +43,39 @@ namespace {
 
 constexpr int kRows = 128;                        // of a tile of queries, and keys of a tile of keys
 constexpr int kThreads = 384;                    // three warpgroups; 168 registers a thread at launch
-constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
+constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
 static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * 168, "registers");
 constexpr int kCtrlBytes = 512;
 constexpr int kTmemCols = 512;
 constexpr uint32_t kColO = 256;
-constexpr float kLazy = 8.f;
+constexpr float kLazy = 8.f, kMost = 14.f;        // log2 of a weight: from where the maximum follows, and the largest
+constexpr int kMinChunk = 8;                      // tiles of keys: the shortest piece that an item is cut into
+constexpr int kFirstGroups = 6;                   // of 16 keys, whose weights are announced first
+constexpr int kReaders = 11;                      // warps that read an item
+constexpr int kSignals = 8;                       // more than the products can be ahead of the copies: stages / 2 + 1
 
 template <int D>
-constexpr int stages() { return D == 128 ? 5 : 8; }
+constexpr int stages() { return D == 128 ? 4 : 8; }
+constexpr int kStageOut = 32 * 128;               // a warp's output on its way: 32 rows x 128 bytes
 template <int D>
-constexpr int smem_bytes() { return (2 + stages<D>()) * kRows * D * 2 + kCtrlBytes; }
+constexpr int smem_bytes() { return (2 + stages<D>()) * kRows * D * 2 + 8 * kStageOut + kCtrlBytes; }
+
+// The queries of one sequence that a CTA works on, and the part of the sequence's keys.
+struct alignas(16) Item {
+  int b, n, m;          // sequence, its queries and keys; b < 0: no more items
+  int first;            // first query of the item in its sequence
+  int row0, key0;       // where the sequence begins in q and in packed keys
+  int lo, hi;           // tiles of keys
+  int slot, pieces;     // pieces > 1: place of this piece's partial results (times key heads)
+  int kv, pad;
+  struct {
+    int skip;           // steps that a tile of rows sits out at the beginning; all of them where it has no rows or sees no key
+    int cols;           // how many keys of its first step's tile it sees
+  } part[2];
+};
+struct Header {
+  int units, next, joins, pad;
+};
 
 struct PrefillParams {
   void* out;
@@ -54,22 +83,107 @@ struct PrefillParams {
   int64_t table_stride;
   int tokens, key_tokens, sequences, heads, kv_heads, group, dim, pages, page_size, table_width;
   int tile_tokens;      // queries of a tile: 128 / group
+  int group_inverse;    // row / group = row * group_inverse >> 16
   int box_rows;
   int causal;
   float scale_log2;
+  int split, sms;
+  Header* header;       // NULL: a CTA for each item, no list
+  Item* units;          // the list; kv and part are not set, nor in `joins` lo and hi
+  Item* joins;          // items that were cut: slot of their first piece
+  float* part_o;        // [slot][key head][2 tiles x 128 rows][D]
+  float2* part_ml;      // maximum, sum
   int* status;
-};
-
-// The queries of one sequence that a CTA works on, and the sequence's keys.
-struct Item {
-  int b, n, m;          // sequence, its queries and keys
-  int first;            // first query of the CTA in its sequence
-  int row0, key0;       // where the sequence begins in q and in packed keys
 };
 
 __device__ __forceinline__ int begin_of(const PrefillParams& p, int b) { return min(max(p.cu_q[b], 0), p.tokens); }
 __device__ __forceinline__ int queries_of(const PrefillParams& p, int b) {
   return max(min(p.cu_q[b + 1], p.tokens) - begin_of(p, b), 0);
+}
+__device__ __forceinline__ int items_of(const PrefillParams& p, int n) {
+  return (n + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
+}
+// Keys that query i sees: [0, seen).
+__device__ __forceinline__ int seen_by(const PrefillParams& p, const Item& it, int i) {
+  return max(0, p.causal ? min(it.m, i + 1 + it.m - it.n) : it.m);
+}
+__device__ __forceinline__ Item sequence_of(const PrefillParams& p, int b) {
+  Item it{};
+  it.b = b, it.n = queries_of(p, b), it.row0 = begin_of(p, b), it.key0 = p.cu_k[b], it.pieces = 1;
+  int64_t m = p.cu_k[b + 1] - static_cast<int64_t>(it.key0);
+  if (p.page_size > 0) m = min(m, static_cast<int64_t>(p.table_width) * p.page_size);
+  else m = it.key0 < 0 ? 0 : min(m, static_cast<int64_t>(p.key_tokens) - it.key0);
+  it.m = static_cast<int>(min(max(m, int64_t{0}), static_cast<int64_t>(INT_MAX - kRows)));
+  return it;
+}
+__device__ __forceinline__ void set_item(const PrefillParams& p, Item& it, int index) {
+  it.first = index * 2 * p.tile_tokens;
+  it.lo = 0;
+  it.hi = (seen_by(p, it, min(it.first + 2 * p.tile_tokens, it.n) - 1) + kRows - 1) / kRows;
+}
+
+// Lists the items by falling number of keys.  One block: a warp takes a sequence, a lane an item.
+constexpr int kPlanThreads = 1024, kBuckets = 1024;
+__global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillParams p) {
+  __shared__ int count[kBuckets], sums[32], slots, joins;
+  __shared__ unsigned long long work;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  count[threadIdx.x] = 0;
+  if (threadIdx.x == 0) slots = joins = 0, work = 0;
+  ptx::grid_launch_dependents();
+  ptx::grid_dependency_wait();
+  __syncthreads();
+  unsigned long long mine = 0;
+  for (int b = warp; b < p.sequences; b += 32) {
+    Item it = sequence_of(p, b);
+    for (int i = lane; i < items_of(p, it.n); i += 32) {
+      set_item(p, it, i);
+      mine += it.hi;
+    }
+  }
+  if (mine > 0) atomicAdd(&work, mine);
+  __syncthreads();
+  const long long share = (static_cast<long long>(work) * p.kv_heads + p.sms - 1) / p.sms;
+  const int chunk = p.split ? static_cast<int>(min(max(share, static_cast<long long>(kMinChunk)), static_cast<long long>(INT_MAX))) : INT_MAX;
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int b = warp; b < p.sequences; b += 32) {
+      Item it = sequence_of(p, b);
+      for (int i = lane; i < items_of(p, it.n); i += 32) {
+        set_item(p, it, i);
+        const int all = it.hi;
+        it.pieces = all > chunk ? (all + chunk - 1) / chunk : 1;
+        if (pass == 1 && it.pieces > 1) {
+          it.slot = atomicAdd(&slots, it.pieces);
+          p.joins[atomicAdd(&joins, 1)] = it;
+        }
+        for (int c = 0; c < it.pieces; ++c) {
+          it.lo = static_cast<int>(static_cast<long long>(all) * c / it.pieces);
+          it.hi = static_cast<int>(static_cast<long long>(all) * (c + 1) / it.pieces);
+          const int at = atomicAdd(&count[kBuckets - 1 - min(it.hi - it.lo, kBuckets - 1)], 1);
+          if (pass == 1) {
+            p.units[at] = it;
+            ++it.slot;
+          }
+        }
+      }
+    }
+    __syncthreads();
+    if (pass == 0) {      // where each bucket begins
+      const int own = count[threadIdx.x];
+      int upto = own;
+      for (int x = 1; x < 32; x *= 2) {
+        const int o = __shfl_up_sync(~0u, upto, x);
+        if (lane >= x) upto += o;
+      }
+      if (lane == 31) sums[warp] = upto;
+      __syncthreads();
+      for (int w = 0; w < warp; ++w) upto += sums[w];
+      count[threadIdx.x] = upto - own;
+      if (threadIdx.x == kPlanThreads - 1) p.header->units = upto, p.header->next = 0;
+      __syncthreads();
+    }
+  }
+  if (threadIdx.x == 0) p.header->joins = joins;
 }
 
 template <typename T, int D>
@@ -82,19 +196,21 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
   constexpr int kStages = stages<D>();
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* ring = smem + 2 * kTileBytes;
-  uint8_t* ctrl = ring + kStages * kTileBytes;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(ctrl);   // [stages] a K or V tile is there
-  uint64_t* free_bar = full_bar + kStages;                  // [4], in turn: products up to a step are done
-  uint64_t* s_bar = free_bar + 4;                           // [2] scores of a tile are there
-  uint64_t* p_bar = s_bar + 2;                              // [2][2] its weights are, of half of the keys
-  uint64_t* o_bar = p_bar + 4;                              // all products are done
-  uint64_t* q_bar = o_bar + 1;
-  uint64_t* tail_bar = q_bar + 1;                           // the last V tile, before its end is zeroed
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail_bar + 1);
+  uint8_t* out_stage = ring + kStages * kTileBytes;
+  uint8_t* ctrl = out_stage + 8 * kStageOut;
+  Item* items = reinterpret_cast<Item*>(ctrl);              // [2]
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(items + 2);   // [stages] a K or V tile is there
+  uint64_t* free_bar = full_bar + kStages;                  // [signals], in turn: products up to a step are done
+  uint64_t* s_bar = free_bar + kSignals;                           // [2] scores of a tile are there
+  uint64_t* p_bar = s_bar + 2;                              // [2][2] its weights are, of the first keys and the others
+  uint64_t* o_bar = p_bar + 4;                              // [2] all products of an item are done
+  uint64_t* q_bar = o_bar + 2;
+  uint64_t* tail_bar = q_bar + 1;                           // a last V tile, before its end is cleared
+  uint64_t* item_bar = tail_bar + 1;                        // [2] an item is there
+  uint64_t* read_bar = item_bar + 2;                        // [2] all have read it
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(read_bar + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* scan = reinterpret_cast<int*>(tmem_slot + 2);        // [warps]
-  Item* s_item = reinterpret_cast<Item*>(scan + kThreads / 32);
-  static_assert(8 * (kStages + 13) + 8 + kThreads / 8 + sizeof(Item) <= kCtrlBytes, "control words");
+  static_assert(2 * sizeof(Item) + 8 * (kStages + kSignals + 14) + 8 <= kCtrlBytes, "control words");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t smem_base = ptx::smem_u32(smem), ring_base = smem_base + 2 * kTileBytes;
@@ -104,17 +220,18 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
   }
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) ptx::mbar_init(ptx::smem_u32(full_bar + s), 1);
-    for (int e = 0; e < 4; ++e) ptx::mbar_init(ptx::smem_u32(free_bar + e), 1);
+    for (int e = 0; e < kSignals; ++e) ptx::mbar_init(ptx::smem_u32(free_bar + e), 1);
     for (int t = 0; t < 2; ++t) {
       ptx::mbar_init(ptx::smem_u32(s_bar + t), 1);
       ptx::mbar_init(ptx::smem_u32(p_bar + 2 * t), 4);
       ptx::mbar_init(ptx::smem_u32(p_bar + 2 * t + 1), 4);
+      ptx::mbar_init(ptx::smem_u32(item_bar + t), 1);
+      ptx::mbar_init(ptx::smem_u32(read_bar + t), kReaders);
+      ptx::mbar_init(ptx::smem_u32(o_bar + t), 1);
     }
-    ptx::mbar_init(ptx::smem_u32(o_bar), 1);
     ptx::mbar_init(ptx::smem_u32(q_bar), 1);
     ptx::mbar_init(ptx::smem_u32(tail_bar), 1);
     *abort_flag = 0;
-    s_item->b = -1;
     ptx::fence_mbar_init();
     ptx::tma_prefetch_desc(&tmap_q);
     ptx::tma_prefetch_desc(&tmap_k);
@@ -124,92 +241,115 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     ptx::tmem_alloc(ptx::smem_u32(tmem_slot), kTmemCols);
     ptx::tmem_relinquish();
   }
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  ptx::tc_fence_after_sync();
   ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
-
-  // Which queries: items of two tiles, sequence by sequence; the last one, with the most keys, is taken first.
-  const int kv = blockIdx.x % p.kv_heads, per_item = 2 * p.tile_tokens;
-  {
-    const int per = (p.sequences + kThreads - 1) / kThreads, b0 = threadIdx.x * per, b1 = min(b0 + per, p.sequences);
-    int mine = 0;
-    for (int b = b0; b < b1; ++b) mine += (queries_of(p, b) + per_item - 1) / per_item;
-    int upto = mine;
-    for (int x = 1; x < 32; x *= 2) {
-      const int o = __shfl_up_sync(~0u, upto, x);
-      if (lane >= x) upto += o;
-    }
-    if (lane == 31) scan[warp] = upto;
-    ptx::tc_fence_before_sync();
-    __syncthreads();
-    ptx::tc_fence_after_sync();
-    int total = 0;
-    for (int w = 0; w < kThreads / 32; ++w) {
-      if (w == warp) upto += total;
-      total += scan[w];
-    }
-    const int item = total - 1 - static_cast<int>(blockIdx.x) / p.kv_heads;
-    int first = upto - mine;
-    if (item >= first && item < upto) {      // one thread, or none
-      int b = b0, n;
-      while (true) {
-        n = queries_of(p, b);
-        const int items = (n + per_item - 1) / per_item;
-        if (item < first + items) break;
-        first += items;
-        ++b;
-      }
-      Item it;
-      it.b = b, it.n = n, it.first = (item - first) * per_item, it.row0 = begin_of(p, b);
-      it.key0 = p.cu_k[b];
-      int64_t m = p.cu_k[b + 1] - static_cast<int64_t>(it.key0);
-      if (p.page_size > 0) m = min(m, static_cast<int64_t>(p.table_width) * p.page_size);
-      else m = it.key0 < 0 ? 0 : min(m, static_cast<int64_t>(p.key_tokens) - it.key0);
-      it.m = static_cast<int>(min(max(m, int64_t{0}), static_cast<int64_t>(INT_MAX - kRows)));
-      *s_item = it;
-    }
-    __syncthreads();
-  }
-  const Item it = *s_item;
   const uint32_t tmem_base = *tmem_slot;      // all columns: 0, which the products' constants rely on
-  if (tmem_base != 0 && threadIdx.x == 0) atomicCAS(p.status, 0, 0x200);
+  if (tmem_base != 0 && threadIdx.x == 0) {
+    atomicCAS(p.status, 0, 0x200);
+    *abort_flag = 1;
+  }
 
-  if (it.b >= 0 && tmem_base == 0) {
-    // Keys that query i sees: [0, seen(i)).
-    const auto seen = [&](int i) { return max(0, p.causal ? min(it.m, i + 1 + it.m - it.n) : it.m); };
-    int tiles[2], steps = 0;      // of keys
+  bool alive = true;
+  int turn = 0;
+  const auto fetch = [&](Item& it) -> bool {
+    const int slot = turn & 1;
+    if (alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(item_bar + slot), (turn >> 1) & 1, abort_flag));
+    it = items[slot];
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(read_bar + slot));
+    ++turn;
+    return alive && it.b >= 0;
+  };
+  if (warp == 10) {
+    ptx::lower_registers<kOtherRegs>();
+    // ---------------------------------------------------------------- items
+    for (int k = 0;; ++k) {
+      Item it{};
+      it.b = -1;
+      if (p.header != nullptr) {
+        int at = lane == 0 ? atomicAdd(&p.header->next, 1) : 0;
+        at = __shfl_sync(~0u, at, 0);
+        if (at / p.kv_heads < *const_cast<const volatile int*>(&p.header->units)) {
+          it = p.units[at / p.kv_heads];
+          it.kv = at % p.kv_heads;
+        }
+      } else if (k == 0) {
+        // the blockIdx.x / kv_heads-th item of all sequences
+        int before = static_cast<int>(blockIdx.x) / p.kv_heads;
+        for (int b0 = 0; b0 < p.sequences; b0 += 32) {
+          const int own = b0 + lane < p.sequences ? items_of(p, queries_of(p, b0 + lane)) : 0;
+          int upto = own;
+          for (int x = 1; x < 32; x *= 2) {
+            const int o = __shfl_up_sync(~0u, upto, x);
+            if (lane >= x) upto += o;
+          }
+          const uint32_t over = __ballot_sync(~0u, upto > before);
+          if (over != 0) {
+            const int l = __ffs(over) - 1;
+            before -= __shfl_sync(~0u, upto - own, l);
+            it = sequence_of(p, b0 + l);
+            set_item(p, it, before);
+            it.kv = static_cast<int>(blockIdx.x) % p.kv_heads;
+            break;
+          }
+          before -= __shfl_sync(~0u, upto, 31);
+        }
+      }
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int from = it.first + t * p.tile_tokens, to = min(from + p.tile_tokens, it.n);
-      tiles[t] = from < to ? (seen(to - 1) + kRows - 1) / kRows : 0;
-      steps = max(steps, tiles[t]);
+      for (int t = 0; t < 2; ++t) {
+        const int from = it.first + t * p.tile_tokens, to = min(from + p.tile_tokens, it.n);
+        const int seen = from < to ? seen_by(p, it, to - 1) : 0, steps = it.hi - it.lo;
+        it.part[t].skip = min(max(it.hi - (seen + kRows - 1) / kRows, 0), steps);
+        it.part[t].cols = min(seen - (it.hi - 1 - it.part[t].skip) * kRows, kRows);
+      }
+      if (k >= 2 && alive)
+        alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(read_bar + (k & 1)), ((k >> 1) - 1) & 1, abort_flag));
+      if (lane == 0 && alive) {
+        items[k & 1] = it;
+        ptx::mbar_arrive(ptx::smem_u32(item_bar + (k & 1)));
+      }
+      if (it.b < 0 || !alive) break;
     }
-    const int skip[2] = {steps - tiles[0], steps - tiles[1]};     // the last tiles of keys that a tile of rows does not see
-    const bool tail = steps * kRows > it.m;                        // the last tile of keys is not full
-
-    if (warp == 9) {
-      ptx::lower_registers<kOtherRegs>();
-      // ---------------------------------------------------------------- Q, K and V
-      bool alive = true;
-      if (lane == 0 && steps > 0) {
-        const uint32_t bar = ptx::smem_u32(q_bar), rows = p.tile_tokens * p.group * 128;
-        ptx::mbar_arrive_expect_tx(bar, rows * kHalves * ((tiles[0] > 0) + (tiles[1] > 0)));
+  } else if (warp == 9) {
+    ptx::lower_registers<kOtherRegs>();
+    // ---------------------------------------------------------------- Q, K and V
+    const int boxes = kRows / p.box_rows;
+    int stage = 0, freed = 0, signal = 0, q_free = -1;
+    int holder = -1;      // lane l: the signal that frees place l of the ring
+    uint32_t phase = 0, tails = 0, queries = 0;
+    const auto wait_for = [&](int event) {
+      for (; freed <= event; ++freed)
+        if (alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(free_bar + (freed & (kSignals - 1))), (freed / kSignals) & 1, abort_flag));
+    };
+    Item it;
+    while (fetch(it)) {
+      const int steps = it.hi - it.lo;
+      if (steps == 0) continue;
+      const bool any[2] = {it.part[0].skip < steps, it.part[1].skip < steps}, tail = it.hi * kRows > it.m;
+      wait_for(q_free);      // the scores of the item before are done
+      if (lane == 0 && alive) {
+        const uint32_t bar = ptx::smem_u32(q_bar);
+        ptx::mbar_arrive_expect_tx(bar, p.tile_tokens * p.group * 128 * kHalves * (any[0] + any[1]));
+#pragma unroll
         for (int t = 0; t < 2; ++t)
-          for (int h = 0; h < kHalves && tiles[t] > 0; ++h)
-            ptx::tma_load_4d(smem_base + t * kTileBytes + h * kHalfBytes, &tmap_q, bar, h * 64, 0, kv,
+          for (int h = 0; h < kHalves && any[t]; ++h)
+            ptx::tma_load_4d(smem_base + t * kTileBytes + h * kHalfBytes, &tmap_q, bar, h * 64, 0, it.kv,
                              it.row0 + it.first + t * p.tile_tokens);
       }
       __syncwarp();
-      const int boxes = kRows / p.box_rows;
+      ++queries;
       const int32_t* table = p.page_size > 0 ? p.tables + it.b * p.table_stride : nullptr;
-      int stage = 0, freed = 0, page = 0;
-      uint32_t phase = 0;
+      int page = 0;
       for (int s = 0; s < steps; ++s) {
-        const int begin = (steps - 1 - s) * kRows;
+        const int begin = (it.hi - 1 - s) * kRows;
         int at = it.key0 + begin, held = 1, mine = 0;
         if (p.page_size > 0) {
           // pages of the next 32 boxes at a time, from the last key backwards
           if (s * boxes % 32 == 0) {
-            const int64_t pos = static_cast<int64_t>(steps) * kRows - static_cast<int64_t>(s * boxes + lane + 1) * p.box_rows;
+            const int64_t pos = static_cast<int64_t>(it.hi) * kRows - static_cast<int64_t>(s * boxes + lane + 1) * p.box_rows;
             page = 0;
             if (pos >= 0 && pos < it.m) {
               page = table[pos / p.page_size];
@@ -225,212 +365,354 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          // Tile n = 2 s + x takes the place of tile n - kStages: the first key tile is free with the first signal, and the
-          // values of step e - 1 and the keys of step e with signal e.
-          const int need = (2 * s + x - kStages + 1) >> 1;
-          for (; freed <= need; ++freed)
-            if (alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(free_bar + (freed & 3)), (freed >> 2) & 1, abort_flag));
-          const uint32_t bar = ptx::smem_u32(x == 1 && s == 0 && tail ? tail_bar : full_bar + stage);
+          wait_for(__shfl_sync(~0u, holder, stage));
+          const bool last_values = x == 1 && s == 0 && tail;
+          const uint32_t bar = ptx::smem_u32(last_values ? tail_bar : full_bar + stage);
           if (lane == 0 && alive) ptx::mbar_arrive_expect_tx(bar, held * p.box_rows * D * 2);
           __syncwarp();
           if (lane < held && alive)
             for (int h = 0; h < kHalves; ++h)
               ptx::tma_load_4d(ring_base + stage * kTileBytes + h * kHalfBytes + lane * p.box_rows * 128,
-                               x == 0 ? &tmap_k : &tmap_v, bar, h * 64, kv, at, mine);
+                               x == 0 ? &tmap_k : &tmap_v, bar, h * 64, it.kv, at, mine);
+          if (last_values) ++tails;
+          // signals of an item: the first scores; then each step's values together with the next one's scores
+          if (lane == stage) holder = signal + s + x;
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1u;
           }
         }
       }
-      __syncwarp();
-      if (lane == 0) {
-        if (*abort_flag != 0) ptx::drain_ring(full_bar, kStages, stage, phase);
-        if (*abort_flag != 0) ptx::drain_ring(q_bar, steps > 0 ? 1 + tail : 0, 2, 0);      // and the tail's barrier
-      }
-    } else if (warp == 8) {
-      ptx::lower_registers<kOtherRegs>();
-      // ---------------------------------------------------------------- products
-      // The whole warp walks and one lane issues.
-      constexpr uint32_t ab = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-      const uint32_t idesc_s = ptx::umma_idesc(1u, ab, kRows, kRows);
-      const uint32_t idesc_o = ptx::umma_idesc(1u, ab, kRows, D) | ptx::kIdescMnMajorB;
-      const uint64_t q_desc = ptx::umma_desc_k_sw128(smem_base), k_desc = ptx::umma_desc_k_sw128(ring_base);
-      const uint64_t v_desc = ptx::umma_desc_mn_sw128(ring_base, kHalfBytes);
-      const bool one = ptx::elect_one();
-      bool ok = true;
-      const auto scores = [&](int t, int at) {
-        const uint64_t q = q_desc + t * (kTileBytes >> 4), keys = k_desc + at * (kTileBytes >> 4);
+      q_free = signal + steps - 1;
+      signal += steps + 1;
+    }
+    __syncwarp();
+    if (lane == 0) {
+      if (*abort_flag != 0) ptx::drain_ring(full_bar, kStages, stage, phase);
+      if (*abort_flag != 0 && tails > 0) ptx::drain_ring(tail_bar, 1, 1, (tails - 1) & 1);
+      if (*abort_flag != 0 && queries > 0) ptx::drain_ring(q_bar, 1, 1, (queries - 1) & 1);
+    }
+  } else if (warp == 8) {
+    ptx::lower_registers<kOtherRegs>();
+    // ---------------------------------------------------------------- products
+    // The whole warp walks and one lane issues.
+    constexpr uint32_t ab = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    const uint32_t idesc_s = ptx::umma_idesc(1u, ab, kRows, kRows);
+    const uint32_t idesc_o = ptx::umma_idesc(1u, ab, kRows, D) | ptx::kIdescMnMajorB;
+    const uint64_t q_desc = ptx::umma_desc_k_sw128(smem_base), k_desc = ptx::umma_desc_k_sw128(ring_base);
+    const uint64_t v_desc = ptx::umma_desc_mn_sw128(ring_base, kHalfBytes);
+    const bool one = ptx::elect_one();
+    const auto scores = [&](int t, int at, uint32_t idesc) {
+      const uint64_t q = q_desc + t * (kTileBytes >> 4), keys = k_desc + at * (kTileBytes >> 4);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const int off = ((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4;
-          ptx::umma_f16_ss_by(one && ok, t * kRows, q + off, keys + off, idesc_s, k > 0);
-        }
-        ptx::umma_commit_by(one && ok, ptx::smem_u32(s_bar + t));
-      };
-      int stage = 1;
-      uint32_t phase = 0;
-      if (steps > 0)
-        ok = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(q_bar), 0, abort_flag) &&
-                           ptx::mbar_wait(ptx::smem_u32(full_bar), 0, abort_flag));
+      for (int k = 0; k < D / 16; ++k) {
+        const int off = ((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4;
+        ptx::umma_f16_ss_by(one && alive, t * kRows, q + off, keys + off, idesc, k > 0);
+      }
+      ptx::umma_commit_by(one && alive, ptx::smem_u32(s_bar + t));
+    };
+    int stage = 0, signal = 0;
+    uint32_t phase = 0, q_phase = 0, p_phase[2] = {0, 0};
+    Item it;
+    while (fetch(it)) {
+      const int steps = it.hi - it.lo;
+      if (steps == 0) continue;
+      // the first tile of keys of a tile of rows counts up to the last one seen, in sixteens
+      const int groups_first[2] = {(it.part[0].cols + 15) >> 4, (it.part[1].cols + 15) >> 4};
+      const uint32_t idesc_first[2] = {ptx::umma_idesc(1u, ab, kRows, groups_first[0] * 16),
+                                       ptx::umma_idesc(1u, ab, kRows, groups_first[1] * 16)};
+      if (alive)
+        alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(q_bar), q_phase, abort_flag) &&
+                              ptx::mbar_wait(ptx::smem_u32(full_bar + stage), phase, abort_flag));
+      q_phase ^= 1u;
       ptx::tc_fence_after_sync();
 #pragma unroll
       for (int t = 0; t < 2; ++t)
-        if (tiles[t] > 0 && skip[t] == 0) scores(t, 0);
-      ptx::umma_commit_by(one && ok, ptx::smem_u32(free_bar));
+        if (it.part[t].skip == 0) scores(t, stage, idesc_first[t]);
+      ptx::umma_commit_by(one && alive, ptx::smem_u32(free_bar + (signal++ & (kSignals - 1))));
+      if (++stage == kStages) {
+        stage = 0;
+        phase ^= 1u;
+      }
       for (int s = 0; s < steps; ++s) {
         const int v_stage = stage, k_stage = stage + 1 == kStages ? 0 : stage + 1;
         const uint32_t v_phase = phase, k_phase = k_stage == 0 ? phase ^ 1u : phase;
         const bool more = s + 1 < steps;
         const uint64_t values = v_desc + v_stage * (kTileBytes >> 4);
-        if (ok)
-          ok = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(full_bar + v_stage), v_phase, abort_flag) &&
-                             (!more || ptx::mbar_wait(ptx::smem_u32(full_bar + k_stage), k_phase, abort_flag)));
+        if (alive)
+          alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(full_bar + v_stage), v_phase, abort_flag) &&
+                                (!more || ptx::mbar_wait(ptx::smem_u32(full_bar + k_stage), k_phase, abort_flag)));
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          if (s >= skip[t]) {
+          if (s >= it.part[t].skip) {
+            const int groups = s == it.part[t].skip ? groups_first[t] : kRows / 16;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              if (ok) ok = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(p_bar + 2 * t + c), (s - skip[t]) & 1, abort_flag));
+              if (alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(p_bar + 2 * t + c), p_phase[t], abort_flag));
               ptx::tc_fence_after_sync();
 #pragma unroll
-              for (int i = 0; i < kRows / 32; ++i) {
-                const int k = c * (kRows / 32) + i;
-                ptx::umma_f16_ts_by(one && ok, kColO + t * kRows, t * kRows + 8 * k, values + k * (2048 >> 4), idesc_o,
-                                    s > skip[t] || k > 0);
-              }
+              for (int k = c * kFirstGroups; k < (c == 0 ? kFirstGroups : kRows / 16); ++k)
+                ptx::umma_f16_ts_by(one && alive && k < groups, kColO + t * kRows, t * kRows + 8 * k, values + k * (2048 >> 4),
+                                    idesc_o, s > it.part[t].skip || k > 0);
             }
+            p_phase[t] ^= 1u;
+            if (!more) ptx::umma_commit_by(one && alive, ptx::smem_u32(o_bar + t));
           }
-          if (more && s + 1 >= skip[t]) scores(t, k_stage);
+          if (more && s + 1 >= it.part[t].skip) scores(t, k_stage, s + 1 == it.part[t].skip ? idesc_first[t] : idesc_s);
         }
-        ptx::umma_commit_by(one && ok, more ? ptx::smem_u32(free_bar + ((s + 1) & 3)) : ptx::smem_u32(o_bar));
-        for (int x = 0; x < 2; ++x)
+        ptx::umma_commit_by(one && alive, ptx::smem_u32(free_bar + (signal++ & (kSignals - 1))));
+        for (int x = 0; x < 1 + more; ++x)
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1u;
           }
       }
-    } else if (warp >= 8) {
-      ptx::lower_registers<kOtherRegs>();
-    } else {
-      ptx::raise_registers<kSoftmaxRegs>();
-      // ---------------------------------------------------------------- softmax
-      const int t = warp >> 2, row = (warp & 3) * 32 + lane;
-      const int query = it.first + t * p.tile_tokens + row / p.group;
-      const bool real = row < p.tile_tokens * p.group && query < it.n;
-      const int limit = real ? seen(query) : 0;
-      const int first_limit = seen(it.first + t * p.tile_tokens);     // the fewest keys of a row
-      const uint32_t lanes = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-      const uint32_t col_s = lanes + t * kRows, col_o = lanes + kColO + t * kRows;
-      bool alive = true;
-      if (warp == 4 && tail) {
-        // Behind the last key the last V tile holds another sequence's rows or whatever the page did; 0 * NaN is NaN.
-        if (alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(tail_bar), 0, abort_flag));
-        const int from = it.m - (steps - 1) * kRows;
-        for (int e = lane; e < (kRows - from) * (D / 8); e += 32) {
+    }
+  } else if (warp == 11) {
+    ptx::lower_registers<kOtherRegs>();
+    // ---------------------------------------------------------------- ends
+    // Behind the last key the last V tile holds another sequence's rows or whatever the page did, and 0 * NaN is NaN: cleared
+    // up to the next multiple of 16, which is what the products read.
+    int stage = 0;
+    uint32_t tails = 0;
+    Item it;
+    while (fetch(it)) {
+      const int steps = it.hi - it.lo;
+      if (steps > 0 && it.hi * kRows > it.m) {
+        if (alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(tail_bar), tails & 1, abort_flag));
+        ++tails;
+        const int place = stage + 1 == kStages ? 0 : stage + 1, from = it.m - (it.hi - 1) * kRows;
+        for (int e = lane; e < (((from + 15) & ~15) - from) * (D / 8); e += 32) {
           const int r = from + e / (D / 8), c = e % (D / 8);
-          *reinterpret_cast<uint4*>(ring + kTileBytes + (c >> 3) * kHalfBytes + r * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+          *reinterpret_cast<uint4*>(ring + place * kTileBytes + (c >> 3) * kHalfBytes + r * 128 + (c & 7) * 16) =
+              make_uint4(0u, 0u, 0u, 0u);
         }
         ptx::fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0 && alive) ptx::mbar_arrive(ptx::smem_u32(full_bar + 1));
+        if (lane == 0 && alive) ptx::mbar_arrive(ptx::smem_u32(full_bar + place));
       }
-      float top = -INFINITY, sum = 0.f;
-      for (int s = skip[t]; s < steps; ++s) {
-        const int turn = s - skip[t];
-        if (alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(s_bar + t), turn & 1, abort_flag));
+      stage = (stage + 2 * steps) % kStages;
+    }
+  } else {
+    ptx::raise_registers<kSoftmaxRegs>();
+    // ---------------------------------------------------------------- softmax
+    const int t = warp >> 2, row = (warp & 3) * 32 + lane;
+    const int row_query = row * p.group_inverse >> 16;      // row / group
+    const uint32_t lanes = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t col_s = lanes + t * kRows, col_o = lanes + kColO + t * kRows;
+    uint8_t* const my_stage = out_stage + warp * kStageOut;
+    const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
+    uint32_t s_phase = 0, o_phase = 0;
+    for (int k = 0;; ++k) {
+      // the item stays where it is, so that it takes no registers; it is given back behind the output
+      const Item& it = items[k & 1];
+      if (alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(item_bar + (k & 1)), (k >> 1) & 1, abort_flag));
+      if (!alive || it.b < 0) break;
+      const int hi = it.hi, steps = hi - it.lo;
+      const int skip = it.part[t].skip, cols = it.part[t].cols;
+      int limit = 0;                                                           // keys that the row sees
+      {
+        const int query = it.first + t * p.tile_tokens + row_query;
+        if (row_query < p.tile_tokens && query < it.n) limit = seen_by(p, it, query);
+      }
+      const int first_limit = seen_by(p, it, it.first + t * p.tile_tokens);     // the fewest keys of a row
+      float top = -INFINITY, sum = 0.f, want = -INFINITY;
+      for (int s = skip; s < steps; ++s) {
+        if (alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(s_bar + t), s_phase, abort_flag));
         if (!alive) break;
+        s_phase ^= 1u;
         ptx::tc_fence_after_sync();
-        float x[kRows];
+        uint32_t x[kRows];
 #pragma unroll
         for (int c = 0; c < 4; ++c)
           ptx::tmem_ld_32x32b_x32(col_s + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(x + 32 * c));
         ptx::tmem_ld_wait();
-        const int begin = (steps - 1 - s) * kRows;
-        if (begin + kRows > first_limit) {
+        const int begin = (hi - 1 - s) * kRows;
+        const bool masked = begin + kRows > first_limit, start = s == skip;
+        const auto mask = [&](int c) {      // columns 32 c on
+          const int rel = limit - begin - 32 * c;
+          const uint32_t sees = rel >= 32 ? ~0u : rel <= 0 ? 0u : (1u << rel) - 1u;
 #pragma unroll
-          for (int c = 0; c < kRows; ++c)
-            if (begin + c >= limit) x[c] = -INFINITY;
+          for (int i = 0; i < 32; ++i) x[32 * c + i] = (sees >> i) & 1u ? x[32 * c + i] : __float_as_uint(-INFINITY);
+        };
+        const auto highest = [&]() -> float {
+          float most[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) most[i] = __uint_as_float(x[i]);
+#pragma unroll
+          for (int c = 4; c + 8 <= kRows; c += 8)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              most[i] = max3(most[i], __uint_as_float(x[c + 2 * i]), __uint_as_float(x[c + 2 * i + 1]));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) most[i] = fmaxf(most[i], __uint_as_float(x[kRows - 4 + i]));
+          return fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * p.scale_log2;
+        };
+        if (masked) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) mask(c);
         }
-        float most[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-        for (int c = 4; c + 8 <= kRows; c += 8)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) most[i] = max3(most[i], x[c + 2 * i], x[c + 2 * i + 1]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) most[i] = fmaxf(most[i], x[kRows - 4 + i]);
-        const float next = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * p.scale_log2;
-        if (turn == 0) {
-          top = next;
-        } else if (__any_sync(~0u, next > top + kLazy)) {
-          const float raised = fmaxf(next, top);
-          const float f = raised == top ? 1.f : exp2_approx(top - raised);
-          top = raised;
+        // Raises the maximum to `to`.  (The scores were issued behind the last product into O, so that is done.)
+        const auto raise = [&](float to) {
+          const float f = to == top ? 1.f : exp2_approx(top - to);
+          top = to;
           sum *= f;
-          // (the scores were issued behind the last product into O, so that is done as well)
+          if (start) return;
+#pragma unroll 1
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t o[16];
+            ptx::tmem_ld_32x32b_x16(col_o + 16 * c, o);
+            ptx::tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            ptx::tmem_st_32x32b_x16(col_o + 16 * c, o);
+          }
+        };
+        if (start)
+          top = highest();
+        else if (__any_sync(~0u, want > top + kLazy))
+          raise(fmaxf(want, top));
+        // The exponential unit gives 16 results a cycle for the SM; every fourth pair goes through the multipliers instead.
+        uint64_t part[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+        float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        uint32_t e16[kRows / 2];
+        // Weights of pairs [from, to), eight at a time; sums, maxima and conversions of eight stand beside the exponentials of the next.
+        const auto weights = [&](int from, int to) {
+          const float base = top == -INFINITY ? 0.f : -top;
+          const uint64_t base2 = pair(base, base);
+          float2 e[2][8];
+#pragma unroll
+          for (int b = from / 8; b <= to / 8; ++b) {
+            if (b < to / 8) {
+              uint64_t arg[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                arg[i] = fma2(pair(__uint_as_float(x[16 * b + 2 * i]), __uint_as_float(x[16 * b + 2 * i + 1])), scale2, base2);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                if (i % 4 == 3) {
+                  e[b & 1][i] = exp2_poly(arg[i]);
+                } else {
+                  const float2 v = unpair(arg[i]);
+                  e[b & 1][i] = make_float2(exp2_approx(v.x), exp2_approx(v.y));
+                }
+              }
+            }
+            if (b > from / 8) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int at = 8 * (b - 1) + i;
+                const float2 v = e[(b - 1) & 1][i];
+                part[i & 1] = add2(part[i & 1], pair(v.x, v.y));
+                e16[at] = pack16<T>(v.x, v.y);
+                if (at < 32) {
+                  most[i & 1] = max3(most[i & 1], __uint_as_float(x[2 * at]), __uint_as_float(x[2 * at + 1]));
+                  most[2 + (i & 1)] = max3(most[2 + (i & 1)], __uint_as_float(x[64 + 2 * at]), __uint_as_float(x[64 + 2 * at + 1]));
+                }
+              }
+            }
+          }
+        };
+        const auto announce = [&](int c) {      // the product of these weights may begin
+          ptx::tmem_st_wait();
+          ptx::tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(p_bar + 2 * t + c));
+        };
+        // The maximum of these scores is not waited for: it is found beside the exponentials of the first half, and counts
+        // from the next step on.  Only where it is out of reach (weights above 2^14) is the half done again.
+        weights(0, 32);
+        want = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * p.scale_log2;
+        if (!start && __any_sync(~0u, want > top + kMost)) {
+          raise(fmaxf(want, top));
+          part[0] = part[1] = pair(0.f, 0.f);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            ptx::tmem_ld_32x32b_x32(col_s + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(x + 32 * c));
+            ptx::tmem_ld_wait();
+            if (masked) mask(c);
+          }
+          weights(0, 32);
+        }
+        ptx::tmem_st_32x32b_x32(col_s, *reinterpret_cast<uint32_t(*)[32]>(e16));
+        // three quarters of the keys first: what is left of the product is then short when the last weights come
+        if (!start || cols > kRows / 2) {      // else no row sees the second half
+          weights(32, 48);
+          ptx::tmem_st_32x32b_x16(col_s + 32, *reinterpret_cast<uint32_t(*)[16]>(e16 + 32));
+        }
+        announce(0);
+        if (!start || cols > kRows / 4 * 3) {
+          weights(48, 64);
+          ptx::tmem_st_32x32b_x16(col_s + 48, *reinterpret_cast<uint32_t(*)[16]>(e16 + 48));
+        }
+        announce(1);
+        const float2 both = unpair(add2(part[0], part[1]));
+        sum += both.x + both.y;
+      }
+      // ---- output
+      const bool any = skip < steps;
+      if (any) {
+        if (alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(o_bar + t), o_phase, abort_flag));
+        if (!alive) break;
+        o_phase ^= 1u;
+      }
+      ptx::tc_fence_after_sync();
+      // 128 bytes of each row at a time, through shared memory: eight lanes write a line of a row together
+      const int to = it.first + t * p.tile_tokens, rows = min(it.n - to, p.tile_tokens) * p.group;      // real ones
+      const auto store = [&](uint8_t* base, int row_bytes, int query_bytes, int from, int bytes) {
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = 4 * i + (lane >> 3), all = (warp & 3) * 32 + r, at = from + (lane & 7) * 16;
+          const uint4 v = *reinterpret_cast<const uint4*>(my_stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+          if (all < rows && at < bytes)
+            *reinterpret_cast<uint4*>(base + all * row_bytes + (all * p.group_inverse >> 16) * query_bytes + at) = v;
+        }
+        __syncwarp();
+      };
+      const auto staged = [&](int i) { return reinterpret_cast<uint4*>(my_stage + lane * 128 + ((i ^ (lane & 7)) << 4)); };
+      if (it.pieces > 1) {
+        const int64_t at = (static_cast<int64_t>(it.slot) * p.kv_heads + it.kv) * 2 * kRows + t * kRows;
+        if (row < rows) p.part_ml[at + row] = make_float2(top, sum);
+        if (any) {
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {
             uint32_t o[32];
             ptx::tmem_ld_32x32b_x32(col_o + 32 * c, o);
             ptx::tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            ptx::tmem_st_32x32b_x32(col_o + 32 * c, o);
+            for (int i = 0; i < 8; ++i) *staged(i) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            store(reinterpret_cast<uint8_t*>(p.part_o + at * D), D * 4, 0, c * 128, D * 4);
           }
         }
-        const float base = top == -INFINITY ? 0.f : top;
-        // The exponential unit gives 16 results a cycle for the SM; every fourth pair goes through the multipliers instead.
-        const uint64_t scale2 = pair(p.scale_log2, p.scale_log2), base2 = pair(-base, -base);
-        uint64_t part[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+      } else {
+        // rows of one query are neighbours; the next query is all heads further
+        uint8_t* base = reinterpret_cast<uint8_t*>(static_cast<T*>(p.out) +
+                                                   (static_cast<int64_t>(it.row0 + to) * p.heads + it.kv * p.group) * p.dim);
+        const float inv = limit > 0 ? 1.f / sum : 0.f;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t w[32];
+        for (int c = 0; c < D / 64; ++c) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const uint64_t arg = fma2(pair(x[64 * c + 2 * i], x[64 * c + 2 * i + 1]), scale2, base2);
-            float2 e;
-            if (i % 4 == 3) {
-              e = exp2_poly(arg);
-            } else {
-              e = unpair(arg);
-              e = make_float2(exp2_approx(e.x), exp2_approx(e.y));
+          for (int h = 0; h < 2; ++h) {
+            uint32_t o[32];
+            if (any) {
+              ptx::tmem_ld_32x32b_x32(col_o + 64 * c + 32 * h, o);
+              ptx::tmem_ld_wait();
             }
-            part[i & 1] = add2(part[i & 1], pair(e.x, e.y));
-            w[i] = pack16<T>(e.x, e.y);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t v[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                v[j] = limit > 0 ? pack16<T>(__uint_as_float(o[8 * i + 2 * j]) * inv, __uint_as_float(o[8 * i + 2 * j + 1]) * inv) : 0u;
+              *staged(4 * h + i) = make_uint4(v[0], v[1], v[2], v[3]);
+            }
           }
-          ptx::tmem_st_32x32b_x32(col_s + 32 * c, w);
-          // the product of this half may begin
-          ptx::tmem_st_wait();
-          ptx::tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(p_bar + 2 * t + c));
-        }
-        const float2 both = unpair(add2(part[0], part[1]));
-        sum += both.x + both.y;
-      }
-      const int head = kv * p.group + row % p.group;
-      uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(p.out) +
-                                            (static_cast<int64_t>(it.row0 + query) * p.heads + head) * p.dim);
-      const bool any = tiles[t] > 0;
-      if (any && alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(o_bar), 0, abort_flag));
-      ptx::tc_fence_after_sync();
-      const float inv = limit > 0 ? 1.f / sum : 0.f;
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        if (any && alive) {
-          ptx::tmem_ld_32x32b_x32(col_o + 32 * c, o);
-          ptx::tmem_ld_wait();
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t w[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            w[k] = limit > 0 ? pack16<T>(__uint_as_float(o[8 * i + 2 * k]) * inv, __uint_as_float(o[8 * i + 2 * k + 1]) * inv) : 0u;
-          if (real && alive && 32 * c + 8 * i < p.dim) out[4 * c + i] = make_uint4(w[0], w[1], w[2], w[3]);
+          store(base, p.dim * 2, (p.heads - p.group) * p.dim * 2, c * 128, p.dim * 2);
         }
       }
+      if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(read_bar + (k & 1)));
+      ptx::tc_fence_before_sync();      // O is read before the next weights are announced
     }
   }
   __syncwarp();
@@ -443,8 +725,75 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
   if (threadIdx.x == 0 && *abort_flag != 0) atomicCAS(p.status, 0, 0x900 | (static_cast<int>(blockIdx.x) << 12));
 }
 
+// The pieces of an item that was cut, in their order: a warp takes a row, a lane four dimensions.
+constexpr int kJoinThreads = 256, kJoinBlocks = 8;      // blocks that share the rows of an item and key head
 template <typename T, int D>
-int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PrefillParams& p, cudaStream_t stream) {
+__global__ void __launch_bounds__(kJoinThreads) attn_prefill_join_kernel(const PrefillParams p) {
+  ptx::grid_launch_dependents();
+  ptx::grid_dependency_wait();
+  if (static_cast<int>(blockIdx.x) >= p.header->joins * p.kv_heads) return;
+  const Item it = p.joins[blockIdx.x / p.kv_heads];
+  const int kv = blockIdx.x % p.kv_heads, lane = threadIdx.x & 31, d = lane * 4;
+  for (int r = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5); r < 2 * kRows; r += kJoinBlocks * (kJoinThreads / 32)) {
+    const int row = r % kRows, query = it.first + r / kRows * p.tile_tokens + row / p.group;
+    if (row >= p.tile_tokens * p.group || query >= it.n) continue;
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int c = 0; c < it.pieces; ++c) {
+      const int64_t at = (static_cast<int64_t>(it.slot + c) * p.kv_heads + kv) * 2 * kRows + r;
+      const float2 ml = p.part_ml[at];
+      // a piece of which the row's tile sees nothing has written no sums
+      const float4 v = d < p.dim && ml.x != -INFINITY ? *reinterpret_cast<const float4*>(p.part_o + at * D + d)
+                                                       : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float n = fmaxf(m, ml.x), base = n == -INFINITY ? 0.f : n;
+      const float f = exp2_approx(m - base), g = exp2_approx(ml.x - base);
+      m = n;
+      l = l * f + ml.y * g;
+      acc.x = acc.x * f + v.x * g, acc.y = acc.y * f + v.y * g;
+      acc.z = acc.z * f + v.z * g, acc.w = acc.w * f + v.w * g;
+    }
+    const float inv = seen_by(p, it, query) > 0 ? 1.f / l : 0.f;
+    const int head = kv * p.group + row % p.group;
+    if (d < p.dim)
+      *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (static_cast<int64_t>(it.row0 + query) * p.heads + head) * p.dim + d) =
+          make_uint2(pack16<T>(acc.x * inv, acc.y * inv), pack16<T>(acc.z * inv, acc.w * inv));
+  }
+}
+
+// What depends on the shapes and the hints alone.
+struct Plan {
+  int per_item, planned, split;
+  int64_t items, units;      // at most
+  size_t joins, ml, o;       // bytes of the workspace in front of each
+  size_t bytes;
+};
+
+Plan make_plan(const b200q_attention& a) {
+  Plan plan{};
+  const int sms = sm_count(), d = a.dim <= 64 ? 64 : 128;
+  plan.per_item = 2 * (kRows / (a.heads / a.kv_heads));
+  // at most one item of each sequence is not full
+  plan.items = std::min<int64_t>(a.tokens, a.tokens / plan.per_item + static_cast<int64_t>(a.sequences));
+  // No item is cut where the longest has no more than an SM's share of all keys, each item having one tile of keys at
+  // least; nor where it is short.
+  const int64_t longest = (static_cast<int64_t>(a.max_k) + kRows - 1) / kRows;
+  plan.split = longest > kMinChunk && a.tokens / plan.per_item * a.kv_heads < sms * longest;
+  plan.planned = plan.split || plan.items * a.kv_heads > sms;
+  plan.units = plan.items + (plan.split ? 2 * sms : 0);
+  if (!plan.planned) return plan;
+  const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  plan.joins = 256 + up(plan.units * sizeof(Item));
+  plan.ml = plan.joins + (plan.split ? up(sms * sizeof(Item)) : 0);
+  // an item that is cut has more than an SM's share, and at most twice as many pieces as shares: 2 pieces an SM
+  plan.o = plan.ml + (plan.split ? up(2 * sms * 2 * kRows * sizeof(float2)) : 0);
+  plan.bytes = plan.o + (plan.split ? static_cast<size_t>(2 * sms) * 2 * kRows * d * sizeof(float) : 0);
+  return plan;
+}
+
+template <typename T, int D>
+int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PrefillParams& p, const Plan& plan,
+           cudaStream_t stream) {
   constexpr int smem = smem_bytes<D>();
   static_assert(smem <= 227 * 1024 && 2 * smem > kSmSharedBytes, "one CTA an SM: it takes all tensor memory");
   static bool attr_set[64] = {false};
@@ -456,26 +805,33 @@ int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, 
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e == cudaSuccess && dev < 64) attr_set[dev] = true;
   }
-  // at most one item of each sequence is not full
-  const int per_item = 2 * p.tile_tokens;
-  const int64_t items = std::min<int64_t>(p.tokens, p.tokens / per_item + static_cast<int64_t>(p.sequences));
-  if (items * p.kv_heads > 0x7fffffff) return B200Q_ERR_BAD_SHAPE;
+  int launches = 1;
+  if (e == cudaSuccess && plan.planned) {
+    e = launch_overlapped(MAX_SHARED, attn_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p);
+    ++launches;
+  }
+  const int64_t ctas = plan.planned ? std::min<int64_t>(p.sms, plan.units * p.kv_heads) : plan.items * p.kv_heads;
   if (e == cudaSuccess)
-    e = launch_overlapped(MAX_SHARED, kern, dim3(static_cast<unsigned>(items * p.kv_heads)), dim3(kThreads), smem, stream, tq,
-                          tk, tv, p);
+    e = launch_overlapped(MAX_SHARED, kern, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), smem, stream, tq, tk, tv, p);
+  if (e == cudaSuccess && plan.split) {
+    e = launch_overlapped(MAX_SHARED, attn_prefill_join_kernel<T, D>, dim3(p.sms, kJoinBlocks), dim3(kJoinThreads), 0, stream, p);
+    ++launches;
+  }
   if (e != cudaSuccess) {
     note_cuda_error(e);
     return B200Q_ERR_LAUNCH;
   }
-  count_launch();
+  count_launch(launches);
   return B200Q_OK;
 }
 
 }  // namespace
 
-size_t attn_prefill_workspace(const b200q_attention&) { return 0; }
+size_t attn_prefill_workspace(const b200q_attention& a) { return make_plan(a).bytes; }
 
-int launch_attn_prefill(const b200q_attention& a, void*, int* status, cudaStream_t stream) {
+int launch_attn_prefill(const b200q_attention& a, void* workspace, int* status, cudaStream_t stream) {
+  const Plan plan = make_plan(a);
+  if (plan.units * a.kv_heads > INT_MAX / 2) return B200Q_ERR_BAD_SHAPE;
   PrefillParams p{};
   p.out = a.out;
   p.cu_q = a.cu_q, p.cu_k = a.cu_k, p.tables = a.tables, p.table_stride = a.table_stride;
@@ -483,11 +839,21 @@ int launch_attn_prefill(const b200q_attention& a, void*, int* status, cudaStream
   p.heads = a.heads, p.kv_heads = a.kv_heads, p.group = a.heads / a.kv_heads, p.dim = a.dim;
   p.pages = a.pages, p.page_size = a.page_size, p.table_width = a.table_width;
   p.tile_tokens = kRows / p.group;
+  p.group_inverse = 65536 / p.group + 1;
   p.box_rows = kRows;
   while (a.page_size % p.box_rows != 0) p.box_rows /= 2;
   p.causal = a.causal;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.status = status;
+  p.split = plan.split, p.sms = sm_count();
+  if (plan.planned) {
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    p.header = reinterpret_cast<Header*>(ws);
+    p.units = reinterpret_cast<Item*>(ws + 256);
+    p.joins = reinterpret_cast<Item*>(ws + plan.joins);
+    p.part_ml = reinterpret_cast<float2*>(ws + plan.ml);
+    p.part_o = reinterpret_cast<float*>(ws + plan.o);
+  }
   CUtensorMap tq, tk, tv;
   // queries: [tokens][key heads][group][dim]
   const uint64_t size[4] = {static_cast<uint64_t>(a.dim), static_cast<uint64_t>(p.group), static_cast<uint64_t>(a.kv_heads),
@@ -501,8 +867,8 @@ int launch_attn_prefill(const b200q_attention& a, void*, int* status, cudaStream
     return B200Q_ERR_LAUNCH;
   const bool bf = a.dtype == B200Q_DTYPE_BF16;
   if (a.dim <= 64)
-    return bf ? launch<__nv_bfloat16, 64>(tq, tk, tv, p, stream) : launch<__half, 64>(tq, tk, tv, p, stream);
-  return bf ? launch<__nv_bfloat16, 128>(tq, tk, tv, p, stream) : launch<__half, 128>(tq, tk, tv, p, stream);
+    return bf ? launch<__nv_bfloat16, 64>(tq, tk, tv, p, plan, stream) : launch<__half, 64>(tq, tk, tv, p, plan, stream);
+  return bf ? launch<__nv_bfloat16, 128>(tq, tk, tv, p, plan, stream) : launch<__half, 128>(tq, tk, tv, p, plan, stream);
 }
 
 }  // namespace b200q
