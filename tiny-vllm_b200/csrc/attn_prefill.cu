@@ -45,13 +45,14 @@ constexpr int kRows = 128;                        // of a tile of queries, and k
 constexpr int kThreads = 384;                    // three warpgroups; 168 registers a thread at launch
 constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
 static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * 168, "registers");
-constexpr int kCtrlBytes = 512;
+constexpr int kCtrlBytes = 1024;
 constexpr int kTmemCols = 512;
 constexpr uint32_t kColO = 256;
 constexpr float kLazy = 8.f, kMost = 14.f;        // log2 of a weight: from where the maximum follows, and the largest
 constexpr int kMinChunk = 8;                      // tiles of keys: the shortest piece that an item is cut into
 constexpr int kFirstGroups = 6;                   // of 16 keys, whose weights are announced first
 constexpr int kReaders = 11;                      // warps that read an item
+constexpr int kItems = 4;                         // places for items that are on their way or worked on
 constexpr int kSignals = 8;                       // more than the products can be ahead of the copies: stages / 2 + 1
 
 template <int D>
@@ -87,7 +88,7 @@ struct PrefillParams {
   int box_rows;
   int causal;
   float scale_log2;
-  int split, sms;
+  int split, sms, ctas, most_units;
   Header* header;       // NULL: a CTA for each item, no list
   Item* units;          // the list; kv and part are not set, nor in `joins` lo and hi
   Item* joins;          // items that were cut: slot of their first piece
@@ -96,9 +97,8 @@ struct PrefillParams {
   int* status;
 };
 
-__device__ __forceinline__ int begin_of(const PrefillParams& p, int b) { return min(max(p.cu_q[b], 0), p.tokens); }
-__device__ __forceinline__ int queries_of(const PrefillParams& p, int b) {
-  return max(min(p.cu_q[b + 1], p.tokens) - begin_of(p, b), 0);
+__device__ __forceinline__ int queries_of(const PrefillParams& p, int from, int to) {
+  return max(min(to, p.tokens) - min(max(from, 0), p.tokens), 0);
 }
 __device__ __forceinline__ int items_of(const PrefillParams& p, int n) {
   return (n + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
@@ -107,10 +107,11 @@ __device__ __forceinline__ int items_of(const PrefillParams& p, int n) {
 __device__ __forceinline__ int seen_by(const PrefillParams& p, const Item& it, int i) {
   return max(0, p.causal ? min(it.m, i + 1 + it.m - it.n) : it.m);
 }
-__device__ __forceinline__ Item sequence_of(const PrefillParams& p, int b) {
+__device__ __forceinline__ Item sequence_of(const PrefillParams& p, const int* cu_q, const int* cu_k, int b) {
   Item it{};
-  it.b = b, it.n = queries_of(p, b), it.row0 = begin_of(p, b), it.key0 = p.cu_k[b], it.pieces = 1;
-  int64_t m = p.cu_k[b + 1] - static_cast<int64_t>(it.key0);
+  it.b = b, it.n = queries_of(p, cu_q[b], cu_q[b + 1]), it.row0 = min(max(cu_q[b], 0), p.tokens);
+  it.key0 = cu_k[b], it.pieces = 1;
+  int64_t m = cu_k[b + 1] - static_cast<int64_t>(it.key0);
   if (p.page_size > 0) m = min(m, static_cast<int64_t>(p.table_width) * p.page_size);
   else m = it.key0 < 0 ? 0 : min(m, static_cast<int64_t>(p.key_tokens) - it.key0);
   it.m = static_cast<int>(min(max(m, int64_t{0}), static_cast<int64_t>(INT_MAX - kRows)));
@@ -123,19 +124,25 @@ __device__ __forceinline__ void set_item(const PrefillParams& p, Item& it, int i
 }
 
 // Lists the items by falling number of keys.  One block: a warp takes a sequence, a lane an item.
-constexpr int kPlanThreads = 1024, kBuckets = 1024;
+constexpr int kPlanThreads = 1024, kBuckets = 1024, kPlanCached = 2048;
 __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillParams p) {
-  __shared__ int count[kBuckets], sums[32], slots, joins;
+  __shared__ int count[kBuckets], sums[32], slots, joins, cached[2][kPlanCached];
   __shared__ unsigned long long work;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   count[threadIdx.x] = 0;
   if (threadIdx.x == 0) slots = joins = 0, work = 0;
   ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
+  // the lengths are read three times
+  const int *cu_q = p.cu_q, *cu_k = p.cu_k;
+  if (p.sequences < kPlanCached) {
+    for (int b = threadIdx.x; b <= p.sequences; b += kPlanThreads) cached[0][b] = cu_q[b], cached[1][b] = cu_k[b];
+    cu_q = cached[0], cu_k = cached[1];
+  }
   __syncthreads();
   unsigned long long mine = 0;
-  for (int b = warp; b < p.sequences; b += 32) {
-    Item it = sequence_of(p, b);
+  for (int b = p.split ? warp : p.sequences; b < p.sequences; b += 32) {
+    Item it = sequence_of(p, cu_q, cu_k, b);
     for (int i = lane; i < items_of(p, it.n); i += 32) {
       set_item(p, it, i);
       mine += it.hi;
@@ -143,22 +150,26 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
   }
   if (mine > 0) atomicAdd(&work, mine);
   __syncthreads();
-  const long long share = (static_cast<long long>(work) * p.kv_heads + p.sms - 1) / p.sms;
-  const int chunk = p.split ? static_cast<int>(min(max(share, static_cast<long long>(kMinChunk)), static_cast<long long>(INT_MAX))) : INT_MAX;
+  int chunk = INT_MAX;
+  if (p.split) {
+    const unsigned long long share = (work * p.kv_heads + p.sms - 1) / p.sms;
+    chunk = static_cast<int>(min(max(share, static_cast<unsigned long long>(kMinChunk)), static_cast<unsigned long long>(INT_MAX)));
+  }
   for (int pass = 0; pass < 2; ++pass) {
     for (int b = warp; b < p.sequences; b += 32) {
-      Item it = sequence_of(p, b);
+      Item it = sequence_of(p, cu_q, cu_k, b);
       for (int i = lane; i < items_of(p, it.n); i += 32) {
         set_item(p, it, i);
         const int all = it.hi;
         it.pieces = all > chunk ? (all + chunk - 1) / chunk : 1;
+        const int each = it.pieces > 1 ? all / it.pieces : all, rest = all - each * it.pieces;
         if (pass == 1 && it.pieces > 1) {
           it.slot = atomicAdd(&slots, it.pieces);
           p.joins[atomicAdd(&joins, 1)] = it;
         }
         for (int c = 0; c < it.pieces; ++c) {
-          it.lo = static_cast<int>(static_cast<long long>(all) * c / it.pieces);
-          it.hi = static_cast<int>(static_cast<long long>(all) * (c + 1) / it.pieces);
+          it.lo = c * each + min(c, rest);
+          it.hi = it.lo + each + (c < rest);
           const int at = atomicAdd(&count[kBuckets - 1 - min(it.hi - it.lo, kBuckets - 1)], 1);
           if (pass == 1) {
             p.units[at] = it;
@@ -177,9 +188,18 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
       }
       if (lane == 31) sums[warp] = upto;
       __syncthreads();
-      for (int w = 0; w < warp; ++w) upto += sums[w];
+      if (warp == 0) {
+        int before = sums[lane];
+        for (int x = 1; x < 32; x *= 2) {
+          const int o = __shfl_up_sync(~0u, before, x);
+          if (lane >= x) before += o;
+        }
+        sums[lane] = before;
+      }
+      __syncthreads();
+      if (warp > 0) upto += sums[warp - 1];
       count[threadIdx.x] = upto - own;
-      if (threadIdx.x == kPlanThreads - 1) p.header->units = upto, p.header->next = 0;
+      if (threadIdx.x == kPlanThreads - 1) p.header->units = upto, p.header->next = p.ctas;
       __syncthreads();
     }
   }
@@ -198,19 +218,20 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
   uint8_t* ring = smem + 2 * kTileBytes;
   uint8_t* out_stage = ring + kStages * kTileBytes;
   uint8_t* ctrl = out_stage + 8 * kStageOut;
-  Item* items = reinterpret_cast<Item*>(ctrl);              // [2]
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(items + 2);   // [stages] a K or V tile is there
+  Item* items = reinterpret_cast<Item*>(ctrl);              // [items]
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(items + kItems);   // [stages] a K or V tile is there
   uint64_t* free_bar = full_bar + kStages;                  // [signals], in turn: products up to a step are done
   uint64_t* s_bar = free_bar + kSignals;                           // [2] scores of a tile are there
   uint64_t* p_bar = s_bar + 2;                              // [2][2] its weights are, of the first keys and the others
   uint64_t* o_bar = p_bar + 4;                              // [2] all products of an item are done
   uint64_t* q_bar = o_bar + 2;
   uint64_t* tail_bar = q_bar + 1;                           // a last V tile, before its end is cleared
-  uint64_t* item_bar = tail_bar + 1;                        // [2] an item is there
-  uint64_t* read_bar = item_bar + 2;                        // [2] all have read it
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(read_bar + 2);
+  uint64_t* want_bar = tail_bar + 1;                        // the next item is wanted
+  uint64_t* item_bar = want_bar + 1;                        // [items] an item is there
+  uint64_t* read_bar = item_bar + kItems;                   // [items] all have read it
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(read_bar + kItems);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert(2 * sizeof(Item) + 8 * (kStages + kSignals + 14) + 8 <= kCtrlBytes, "control words");
+  static_assert(kItems * sizeof(Item) + 8 * (kStages + kSignals + 11 + 2 * kItems) + 8 <= kCtrlBytes, "control words");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t smem_base = ptx::smem_u32(smem), ring_base = smem_base + 2 * kTileBytes;
@@ -225,12 +246,15 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       ptx::mbar_init(ptx::smem_u32(s_bar + t), 1);
       ptx::mbar_init(ptx::smem_u32(p_bar + 2 * t), 4);
       ptx::mbar_init(ptx::smem_u32(p_bar + 2 * t + 1), 4);
-      ptx::mbar_init(ptx::smem_u32(item_bar + t), 1);
-      ptx::mbar_init(ptx::smem_u32(read_bar + t), kReaders);
       ptx::mbar_init(ptx::smem_u32(o_bar + t), 1);
+    }
+    for (int k = 0; k < kItems; ++k) {
+      ptx::mbar_init(ptx::smem_u32(item_bar + k), 1);
+      ptx::mbar_init(ptx::smem_u32(read_bar + k), kReaders);
     }
     ptx::mbar_init(ptx::smem_u32(q_bar), 1);
     ptx::mbar_init(ptx::smem_u32(tail_bar), 1);
+    ptx::mbar_init(ptx::smem_u32(want_bar), 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
     ptx::tma_prefetch_desc(&tmap_q);
@@ -255,8 +279,8 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
   bool alive = true;
   int turn = 0;
   const auto fetch = [&](Item& it) -> bool {
-    const int slot = turn & 1;
-    if (alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(item_bar + slot), (turn >> 1) & 1, abort_flag));
+    const int slot = turn % kItems;
+    if (alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(item_bar + slot), (turn / kItems) & 1, abort_flag));
     it = items[slot];
     __syncwarp();
     if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(read_bar + slot));
@@ -269,18 +293,26 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     for (int k = 0;; ++k) {
       Item it{};
       it.b = -1;
+      // The next one is taken when the copies of the one before are on their way: taken earlier, it might be left waiting
+      // while another CTA has nothing to do.
+      if (k > 0 && alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(want_bar), (k - 1) & 1, abort_flag));
       if (p.header != nullptr) {
-        int at = lane == 0 ? atomicAdd(&p.header->next, 1) : 0;
-        at = __shfl_sync(~0u, at, 0);
-        if (at / p.kv_heads < *const_cast<const volatile int*>(&p.header->units)) {
-          it = p.units[at / p.kv_heads];
-          it.kv = at % p.kv_heads;
+        int at = static_cast<int>(blockIdx.x);
+        if (k > 0) at = __shfl_sync(~0u, lane == 0 ? atomicAdd(&p.header->next, 1) : 0, 0);
+        const int unit = at / p.kv_heads;
+        if (unit < p.most_units) {      // (both loads at once)
+          it = p.units[unit];
+          it.kv = at - unit * p.kv_heads;
+          if (unit >= *const_cast<const volatile int*>(&p.header->units)) {      // nothing was written there
+            it = Item{};
+            it.b = -1;
+          }
         }
       } else if (k == 0) {
         // the blockIdx.x / kv_heads-th item of all sequences
         int before = static_cast<int>(blockIdx.x) / p.kv_heads;
         for (int b0 = 0; b0 < p.sequences; b0 += 32) {
-          const int own = b0 + lane < p.sequences ? items_of(p, queries_of(p, b0 + lane)) : 0;
+          const int own = b0 + lane < p.sequences ? items_of(p, queries_of(p, p.cu_q[b0 + lane], p.cu_q[b0 + lane + 1])) : 0;
           int upto = own;
           for (int x = 1; x < 32; x *= 2) {
             const int o = __shfl_up_sync(~0u, upto, x);
@@ -290,7 +322,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
           if (over != 0) {
             const int l = __ffs(over) - 1;
             before -= __shfl_sync(~0u, upto - own, l);
-            it = sequence_of(p, b0 + l);
+            it = sequence_of(p, p.cu_q, p.cu_k, b0 + l);
             set_item(p, it, before);
             it.kv = static_cast<int>(blockIdx.x) % p.kv_heads;
             break;
@@ -305,11 +337,11 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         it.part[t].skip = min(max(it.hi - (seen + kRows - 1) / kRows, 0), steps);
         it.part[t].cols = min(seen - (it.hi - 1 - it.part[t].skip) * kRows, kRows);
       }
-      if (k >= 2 && alive)
-        alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(read_bar + (k & 1)), ((k >> 1) - 1) & 1, abort_flag));
+      if (k >= kItems && alive)
+        alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(read_bar + k % kItems), (k / kItems - 1) & 1, abort_flag));
       if (lane == 0 && alive) {
-        items[k & 1] = it;
-        ptx::mbar_arrive(ptx::smem_u32(item_bar + (k & 1)));
+        items[k % kItems] = it;
+        ptx::mbar_arrive(ptx::smem_u32(item_bar + k % kItems));
       }
       if (it.b < 0 || !alive) break;
     }
@@ -327,7 +359,10 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     Item it;
     while (fetch(it)) {
       const int steps = it.hi - it.lo;
-      if (steps == 0) continue;
+      if (steps == 0) {
+        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(want_bar));
+        continue;
+      }
       const bool any[2] = {it.part[0].skip < steps, it.part[1].skip < steps}, tail = it.hi * kRows > it.m;
       wait_for(q_free);      // the scores of the item before are done
       if (lane == 0 && alive) {
@@ -383,6 +418,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
           }
         }
       }
+      if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(want_bar));
       q_free = signal + steps - 1;
       signal += steps + 1;
     }
@@ -413,14 +449,17 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     };
     int stage = 0, signal = 0;
     uint32_t phase = 0, q_phase = 0, p_phase[2] = {0, 0};
+    // the first tile of keys of a tile of rows counts up to the last one seen, in sixteens
+    const auto groups_first = [&](const Item& it, int t) { return (it.part[t].cols + 15) >> 4; };
+    const auto idesc_first = [&](const Item& it, int t) { return ptx::umma_idesc(1u, ab, kRows, groups_first(it, t) * 16); };
+    const auto fetch_keys = [&](Item& it) -> bool {
+      while (fetch(it))
+        if (it.hi > it.lo) return true;
+      return false;
+    };
     Item it;
-    while (fetch(it)) {
+    while (fetch_keys(it)) {
       const int steps = it.hi - it.lo;
-      if (steps == 0) continue;
-      // the first tile of keys of a tile of rows counts up to the last one seen, in sixteens
-      const int groups_first[2] = {(it.part[0].cols + 15) >> 4, (it.part[1].cols + 15) >> 4};
-      const uint32_t idesc_first[2] = {ptx::umma_idesc(1u, ab, kRows, groups_first[0] * 16),
-                                       ptx::umma_idesc(1u, ab, kRows, groups_first[1] * 16)};
       if (alive)
         alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(q_bar), q_phase, abort_flag) &&
                               ptx::mbar_wait(ptx::smem_u32(full_bar + stage), phase, abort_flag));
@@ -428,7 +467,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       ptx::tc_fence_after_sync();
 #pragma unroll
       for (int t = 0; t < 2; ++t)
-        if (it.part[t].skip == 0) scores(t, stage, idesc_first[t]);
+        if (it.part[t].skip == 0) scores(t, stage, idesc_first(it, t));
       ptx::umma_commit_by(one && alive, ptx::smem_u32(free_bar + (signal++ & (kSignals - 1))));
       if (++stage == kStages) {
         stage = 0;
@@ -445,7 +484,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (s >= it.part[t].skip) {
-            const int groups = s == it.part[t].skip ? groups_first[t] : kRows / 16;
+            const int groups = s == it.part[t].skip ? groups_first(it, t) : kRows / 16;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
               if (alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(p_bar + 2 * t + c), p_phase[t], abort_flag));
@@ -458,7 +497,8 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             p_phase[t] ^= 1u;
             if (!more) ptx::umma_commit_by(one && alive, ptx::smem_u32(o_bar + t));
           }
-          if (more && s + 1 >= it.part[t].skip) scores(t, k_stage, s + 1 == it.part[t].skip ? idesc_first[t] : idesc_s);
+          if (more && s + 1 >= it.part[t].skip)
+            scores(t, k_stage, s + 1 == it.part[t].skip ? idesc_first(it, t) : idesc_s);
         }
         ptx::umma_commit_by(one && alive, ptx::smem_u32(free_bar + (signal++ & (kSignals - 1))));
         for (int x = 0; x < 1 + more; ++x)
@@ -503,61 +543,207 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     uint8_t* const my_stage = out_stage + warp * kStageOut;
     const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
     uint32_t s_phase = 0, o_phase = 0;
+    // 128 bytes of each row at a time go through shared memory: eight lanes write a line of a row together
+    const auto staged = [&](int i) { return reinterpret_cast<uint4*>(my_stage + lane * 128 + ((i ^ (lane & 7)) << 4)); };
+    const auto store = [&](uint8_t* base, int rows, int row_bytes, int query_bytes, int from, int bytes) {
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + (lane >> 3), all = (warp & 3) * 32 + r, at = from + (lane & 7) * 16;
+        const uint4 v = *reinterpret_cast<const uint4*>(my_stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+        if (all < rows && at < bytes)
+          *reinterpret_cast<uint4*>(base + all * row_bytes + (all * p.group_inverse >> 16) * query_bytes + at) = v;
+      }
+      __syncwarp();
+    };
+    // An item's result, where tile t has one; `any`: there are sums.
+    const auto output = [&](const Item& it, bool any, bool sees, float top, float sum) {
+      const int to = it.first + t * p.tile_tokens, rows = min(it.n - to, p.tile_tokens) * p.group;      // real ones
+      if (it.pieces > 1) {
+        const int64_t at = (static_cast<int64_t>(it.slot) * p.kv_heads + it.kv) * 2 * kRows + t * kRows;
+        if (row < rows) p.part_ml[at + row] = make_float2(top, sum);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          if (!any) break;
+          uint32_t o[32];
+          ptx::tmem_ld_32x32b_x32(col_o + 32 * c, o);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) *staged(i) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          store(reinterpret_cast<uint8_t*>(p.part_o + at * D), rows, D * 4, 0, c * 128, D * 4);
+        }
+        return;
+      }
+      // rows of one query are neighbours; the next query is all heads further
+      uint8_t* base = reinterpret_cast<uint8_t*>(static_cast<T*>(p.out) +
+                                                 (static_cast<int64_t>(it.row0 + to) * p.heads + it.kv * p.group) * p.dim);
+      const float inv = 1.f / sum;
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t o[32];
+          if (any) {
+            ptx::tmem_ld_32x32b_x32(col_o + 64 * c + 32 * h, o);
+            ptx::tmem_ld_wait();
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              v[j] = sees ? pack16<T>(__uint_as_float(o[8 * i + 2 * j]) * inv, __uint_as_float(o[8 * i + 2 * j + 1]) * inv) : 0u;
+            *staged(4 * h + i) = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        }
+        store(base, rows, p.dim * 2, (p.heads - p.group) * p.dim * 2, c * 128, p.dim * 2);
+      }
+    };
+    uint32_t x[kRows], e16[kRows / 2];
+    uint64_t part[2];
+    float top = 0.f, most[4];
+    // Weights of pairs [from, to), eight at a time; sums, maxima (of all scores, by pair 32) and conversions of eight stand
+    // beside the exponentials of the next.  The exponential unit gives 16 results a cycle for the SM; every fourth pair
+    // goes through the multipliers instead (8192 tokens: no pair 489 us, every 8th 483, every 4th 473, every 2nd 496).
+    const auto weights = [&](int from, int to) {
+      const float base = top == -INFINITY ? 0.f : -top;
+      const uint64_t base2 = pair(base, base);
+      float2 e[2][8];
+#pragma unroll
+      for (int b = from / 8; b <= to / 8; ++b) {
+        if (b < to / 8) {
+          uint64_t arg[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            arg[i] = fma2(pair(__uint_as_float(x[16 * b + 2 * i]), __uint_as_float(x[16 * b + 2 * i + 1])), scale2, base2);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (i % 4 == 3) {
+              e[b & 1][i] = exp2_poly(arg[i]);
+            } else {
+              const float2 v = unpair(arg[i]);
+              e[b & 1][i] = make_float2(exp2_approx(v.x), exp2_approx(v.y));
+            }
+          }
+        }
+        if (b > from / 8) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int at = 8 * (b - 1) + i;
+            const float2 v = e[(b - 1) & 1][i];
+            part[i & 1] = add2(part[i & 1], pair(v.x, v.y));
+            e16[at] = pack16<T>(v.x, v.y);
+            if (at < 32) {
+              most[i & 1] = max3(most[i & 1], __uint_as_float(x[2 * at]), __uint_as_float(x[2 * at + 1]));
+              most[2 + (i & 1)] = max3(most[2 + (i & 1)], __uint_as_float(x[64 + 2 * at]), __uint_as_float(x[64 + 2 * at + 1]));
+            }
+          }
+        }
+      }
+    };
+    const auto announce = [&](int c) {      // the product of these weights may begin
+      ptx::tmem_st_wait();
+      ptx::tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(p_bar + 2 * t + c));
+    };
+    const auto load = [&](int c) {      // columns 32 c on
+      ptx::tmem_ld_32x32b_x32(col_s + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(x + 32 * c));
+    };
+    // The item whose result is still in O: its place, and this row's statistics.
+    int done = -1;
+    bool done_any = false, done_sees = false;
+    float done_top = 0.f, done_sum = 0.f;
     for (int k = 0;; ++k) {
-      // the item stays where it is, so that it takes no registers; it is given back behind the output
-      const Item& it = items[k & 1];
-      if (alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(item_bar + (k & 1)), (k >> 1) & 1, abort_flag));
-      if (!alive || it.b < 0) break;
-      const int hi = it.hi, steps = hi - it.lo;
-      const int skip = it.part[t].skip, cols = it.part[t].cols;
+      const int slot = k % kItems;
+      const Item& it = items[slot];      // read where it is: it would take registers
+      if (alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(item_bar + slot), (k / kItems) & 1, abort_flag));
+      if (!alive) break;
+      const bool end = it.b < 0;
+      const int hi = it.hi, steps = end ? 0 : hi - it.lo, skip = it.part[t].skip, cols = it.part[t].cols;
+      const bool any = !end && skip < steps;
       int limit = 0;                                                           // keys that the row sees
       {
         const int query = it.first + t * p.tile_tokens + row_query;
-        if (row_query < p.tile_tokens && query < it.n) limit = seen_by(p, it, query);
+        if (!end && row_query < p.tile_tokens && query < it.n) limit = seen_by(p, it, query);
       }
       const int first_limit = seen_by(p, it, it.first + t * p.tile_tokens);     // the fewest keys of a row
-      float top = -INFINITY, sum = 0.f, want = -INFINITY;
-      for (int s = skip; s < steps; ++s) {
+      const auto mask = [&](int c, int begin) {      // columns 32 c on
+        const int rel = limit - begin - 32 * c;
+        const uint32_t sees = rel >= 32 ? ~0u : rel <= 0 ? 0u : (1u << rel) - 1u;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) x[32 * c + i] = (sees >> i) & 1u ? x[32 * c + i] : __float_as_uint(-INFINITY);
+      };
+      float sum = 0.f, want = -INFINITY;
+      top = -INFINITY;
+      if (any) {
+        // ---- first step: the maximum comes first
         if (alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(s_bar + t), s_phase, abort_flag));
         if (!alive) break;
         s_phase ^= 1u;
         ptx::tc_fence_after_sync();
-        uint32_t x[kRows];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          ptx::tmem_ld_32x32b_x32(col_s + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(x + 32 * c));
+        for (int c = 0; c < 4; ++c) load(c);
+        ptx::tmem_ld_wait();
+        const int begin = (hi - 1 - skip) * kRows;
+        if (begin + kRows > first_limit) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) mask(c, begin);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most[i] = __uint_as_float(x[i]);
+#pragma unroll
+        for (int c = 4; c + 8 <= kRows; c += 8)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) most[i] = max3(most[i], __uint_as_float(x[c + 2 * i]), __uint_as_float(x[c + 2 * i + 1]));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most[i] = fmaxf(most[i], __uint_as_float(x[kRows - 4 + i]));
+        top = want = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * p.scale_log2;
+        part[0] = part[1] = pair(0.f, 0.f);
+        weights(0, 32);
+        ptx::tmem_st_32x32b_x32(col_s, *reinterpret_cast<uint32_t(*)[32]>(e16));
+        if (cols > kRows / 2) {      // else no row sees the second half
+          weights(32, 64);
+          ptx::tmem_st_32x32b_x32(col_s + 32, *reinterpret_cast<uint32_t(*)[32]>(e16 + 32));
+        }
+        const float2 both = unpair(add2(part[0], part[1]));
+        sum = both.x + both.y;
+      }
+      if (done >= 0) {
+        // ---- the item before: its last product has had the time of this one's first weights
+        if (done_any) {
+          if (alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(o_bar + t), o_phase, abort_flag));
+          if (!alive) break;
+          o_phase ^= 1u;
+          ptx::tc_fence_after_sync();
+        }
+        output(items[done], done_any, done_sees, done_top, done_sum);
+        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(read_bar + done));
+      }
+      if (end) break;
+      if (any) {
+        announce(0);
+        announce(1);
+      }
+      for (int s = skip + 1; s < steps; ++s) {
+        if (alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(s_bar + t), s_phase, abort_flag));
+        if (!alive) break;
+        s_phase ^= 1u;
+        ptx::tc_fence_after_sync();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) load(c);
         ptx::tmem_ld_wait();
         const int begin = (hi - 1 - s) * kRows;
-        const bool masked = begin + kRows > first_limit, start = s == skip;
-        const auto mask = [&](int c) {      // columns 32 c on
-          const int rel = limit - begin - 32 * c;
-          const uint32_t sees = rel >= 32 ? ~0u : rel <= 0 ? 0u : (1u << rel) - 1u;
-#pragma unroll
-          for (int i = 0; i < 32; ++i) x[32 * c + i] = (sees >> i) & 1u ? x[32 * c + i] : __float_as_uint(-INFINITY);
-        };
-        const auto highest = [&]() -> float {
-          float most[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) most[i] = __uint_as_float(x[i]);
-#pragma unroll
-          for (int c = 4; c + 8 <= kRows; c += 8)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              most[i] = max3(most[i], __uint_as_float(x[c + 2 * i]), __uint_as_float(x[c + 2 * i + 1]));
-#pragma unroll
-          for (int i = 0; i < 4; ++i) most[i] = fmaxf(most[i], __uint_as_float(x[kRows - 4 + i]));
-          return fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * p.scale_log2;
-        };
+        const bool masked = begin + kRows > first_limit;
         if (masked) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) mask(c);
+          for (int c = 0; c < 4; ++c) mask(c, begin);
         }
         // Raises the maximum to `to`.  (The scores were issued behind the last product into O, so that is done.)
         const auto raise = [&](float to) {
           const float f = to == top ? 1.f : exp2_approx(top - to);
           top = to;
           sum *= f;
-          if (start) return;
 #pragma unroll 1
           for (int c = 0; c < D / 16; ++c) {
             uint32_t o[16];
@@ -568,151 +754,37 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             ptx::tmem_st_32x32b_x16(col_o + 16 * c, o);
           }
         };
-        if (start)
-          top = highest();
-        else if (__any_sync(~0u, want > top + kLazy))
-          raise(fmaxf(want, top));
-        // The exponential unit gives 16 results a cycle for the SM; every fourth pair goes through the multipliers instead.
-        uint64_t part[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
-        float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        uint32_t e16[kRows / 2];
-        // Weights of pairs [from, to), eight at a time; sums, maxima and conversions of eight stand beside the exponentials of the next.
-        const auto weights = [&](int from, int to) {
-          const float base = top == -INFINITY ? 0.f : -top;
-          const uint64_t base2 = pair(base, base);
-          float2 e[2][8];
-#pragma unroll
-          for (int b = from / 8; b <= to / 8; ++b) {
-            if (b < to / 8) {
-              uint64_t arg[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                arg[i] = fma2(pair(__uint_as_float(x[16 * b + 2 * i]), __uint_as_float(x[16 * b + 2 * i + 1])), scale2, base2);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                if (i % 4 == 3) {
-                  e[b & 1][i] = exp2_poly(arg[i]);
-                } else {
-                  const float2 v = unpair(arg[i]);
-                  e[b & 1][i] = make_float2(exp2_approx(v.x), exp2_approx(v.y));
-                }
-              }
-            }
-            if (b > from / 8) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const int at = 8 * (b - 1) + i;
-                const float2 v = e[(b - 1) & 1][i];
-                part[i & 1] = add2(part[i & 1], pair(v.x, v.y));
-                e16[at] = pack16<T>(v.x, v.y);
-                if (at < 32) {
-                  most[i & 1] = max3(most[i & 1], __uint_as_float(x[2 * at]), __uint_as_float(x[2 * at + 1]));
-                  most[2 + (i & 1)] = max3(most[2 + (i & 1)], __uint_as_float(x[64 + 2 * at]), __uint_as_float(x[64 + 2 * at + 1]));
-                }
-              }
-            }
-          }
-        };
-        const auto announce = [&](int c) {      // the product of these weights may begin
-          ptx::tmem_st_wait();
-          ptx::tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(p_bar + 2 * t + c));
-        };
+        if (__any_sync(~0u, want > top + kLazy)) raise(fmaxf(want, top));
         // The maximum of these scores is not waited for: it is found beside the exponentials of the first half, and counts
         // from the next step on.  Only where it is out of reach (weights above 2^14) is the half done again.
+        part[0] = part[1] = pair(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most[i] = -INFINITY;
         weights(0, 32);
         want = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * p.scale_log2;
-        if (!start && __any_sync(~0u, want > top + kMost)) {
+        if (__any_sync(~0u, want > top + kMost)) {
           raise(fmaxf(want, top));
           part[0] = part[1] = pair(0.f, 0.f);
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            ptx::tmem_ld_32x32b_x32(col_s + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(x + 32 * c));
+            load(c);
             ptx::tmem_ld_wait();
-            if (masked) mask(c);
+            if (masked) mask(c, begin);
           }
           weights(0, 32);
         }
         ptx::tmem_st_32x32b_x32(col_s, *reinterpret_cast<uint32_t(*)[32]>(e16));
         // three quarters of the keys first: what is left of the product is then short when the last weights come
-        if (!start || cols > kRows / 2) {      // else no row sees the second half
-          weights(32, 48);
-          ptx::tmem_st_32x32b_x16(col_s + 32, *reinterpret_cast<uint32_t(*)[16]>(e16 + 32));
-        }
+        weights(32, 48);
+        ptx::tmem_st_32x32b_x16(col_s + 32, *reinterpret_cast<uint32_t(*)[16]>(e16 + 32));
         announce(0);
-        if (!start || cols > kRows / 4 * 3) {
-          weights(48, 64);
-          ptx::tmem_st_32x32b_x16(col_s + 48, *reinterpret_cast<uint32_t(*)[16]>(e16 + 48));
-        }
+        weights(48, 64);
+        ptx::tmem_st_32x32b_x16(col_s + 48, *reinterpret_cast<uint32_t(*)[16]>(e16 + 48));
         announce(1);
         const float2 both = unpair(add2(part[0], part[1]));
         sum += both.x + both.y;
       }
-      // ---- output
-      const bool any = skip < steps;
-      if (any) {
-        if (alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(o_bar + t), o_phase, abort_flag));
-        if (!alive) break;
-        o_phase ^= 1u;
-      }
-      ptx::tc_fence_after_sync();
-      // 128 bytes of each row at a time, through shared memory: eight lanes write a line of a row together
-      const int to = it.first + t * p.tile_tokens, rows = min(it.n - to, p.tile_tokens) * p.group;      // real ones
-      const auto store = [&](uint8_t* base, int row_bytes, int query_bytes, int from, int bytes) {
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int r = 4 * i + (lane >> 3), all = (warp & 3) * 32 + r, at = from + (lane & 7) * 16;
-          const uint4 v = *reinterpret_cast<const uint4*>(my_stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-          if (all < rows && at < bytes)
-            *reinterpret_cast<uint4*>(base + all * row_bytes + (all * p.group_inverse >> 16) * query_bytes + at) = v;
-        }
-        __syncwarp();
-      };
-      const auto staged = [&](int i) { return reinterpret_cast<uint4*>(my_stage + lane * 128 + ((i ^ (lane & 7)) << 4)); };
-      if (it.pieces > 1) {
-        const int64_t at = (static_cast<int64_t>(it.slot) * p.kv_heads + it.kv) * 2 * kRows + t * kRows;
-        if (row < rows) p.part_ml[at + row] = make_float2(top, sum);
-        if (any) {
-#pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            ptx::tmem_ld_32x32b_x32(col_o + 32 * c, o);
-            ptx::tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) *staged(i) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-            store(reinterpret_cast<uint8_t*>(p.part_o + at * D), D * 4, 0, c * 128, D * 4);
-          }
-        }
-      } else {
-        // rows of one query are neighbours; the next query is all heads further
-        uint8_t* base = reinterpret_cast<uint8_t*>(static_cast<T*>(p.out) +
-                                                   (static_cast<int64_t>(it.row0 + to) * p.heads + it.kv * p.group) * p.dim);
-        const float inv = limit > 0 ? 1.f / sum : 0.f;
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t o[32];
-            if (any) {
-              ptx::tmem_ld_32x32b_x32(col_o + 64 * c + 32 * h, o);
-              ptx::tmem_ld_wait();
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t v[4];
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                v[j] = limit > 0 ? pack16<T>(__uint_as_float(o[8 * i + 2 * j]) * inv, __uint_as_float(o[8 * i + 2 * j + 1]) * inv) : 0u;
-              *staged(4 * h + i) = make_uint4(v[0], v[1], v[2], v[3]);
-            }
-          }
-          store(base, p.dim * 2, (p.heads - p.group) * p.dim * 2, c * 128, p.dim * 2);
-        }
-      }
-      if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(read_bar + (k & 1)));
-      ptx::tc_fence_before_sync();      // O is read before the next weights are announced
+      done = slot, done_any = any, done_sees = limit > 0, done_top = top, done_sum = sum;
     }
   }
   __syncwarp();
@@ -725,8 +797,9 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
   if (threadIdx.x == 0 && *abort_flag != 0) atomicCAS(p.status, 0, 0x900 | (static_cast<int>(blockIdx.x) << 12));
 }
 
-// The pieces of an item that was cut, in their order: a warp takes a row, a lane four dimensions.
-constexpr int kJoinThreads = 256, kJoinBlocks = 8;      // blocks that share the rows of an item and key head
+// The pieces of an item that was cut, in their order: a warp takes a row, a lane four dimensions (and the statistics of every 32nd
+// piece).
+constexpr int kJoinThreads = 256, kJoinBlocks = 2 * kRows / (kJoinThreads / 32);
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) attn_prefill_join_kernel(const PrefillParams p) {
   ptx::grid_launch_dependents();
@@ -734,31 +807,35 @@ __global__ void __launch_bounds__(kJoinThreads) attn_prefill_join_kernel(const P
   if (static_cast<int>(blockIdx.x) >= p.header->joins * p.kv_heads) return;
   const Item it = p.joins[blockIdx.x / p.kv_heads];
   const int kv = blockIdx.x % p.kv_heads, lane = threadIdx.x & 31, d = lane * 4;
-  for (int r = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5); r < 2 * kRows; r += kJoinBlocks * (kJoinThreads / 32)) {
-    const int row = r % kRows, query = it.first + r / kRows * p.tile_tokens + row / p.group;
-    if (row >= p.tile_tokens * p.group || query >= it.n) continue;
-    float m = -INFINITY, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int r = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5), row = r % kRows;
+  const int query = it.first + r / kRows * p.tile_tokens + row / p.group;
+  if (row >= p.tile_tokens * p.group || query >= it.n) return;
+  const auto at = [&](int c) { return (static_cast<int64_t>(it.slot + c) * p.kv_heads + kv) * 2 * kRows + r; };
+  float top = -INFINITY;
+  for (int c = lane; c < it.pieces; c += 32) top = fmaxf(top, p.part_ml[at(c)].x);
+  for (int x = 16; x > 0; x /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
+  const float base = top == -INFINITY ? 0.f : top;
+  float l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int c0 = 0; c0 < it.pieces; c0 += 32) {
+    const float2 ml = c0 + lane < it.pieces ? p.part_ml[at(c0 + lane)] : make_float2(-INFINITY, 0.f);
+    const float weight = exp2_approx(ml.x - base);
+    const bool written = ml.x != -INFINITY;      // a piece of which the row's tile sees nothing has written no sums
+    const int count = min(it.pieces - c0, 32);
 #pragma unroll 4
-    for (int c = 0; c < it.pieces; ++c) {
-      const int64_t at = (static_cast<int64_t>(it.slot + c) * p.kv_heads + kv) * 2 * kRows + r;
-      const float2 ml = p.part_ml[at];
-      // a piece of which the row's tile sees nothing has written no sums
-      const float4 v = d < p.dim && ml.x != -INFINITY ? *reinterpret_cast<const float4*>(p.part_o + at * D + d)
-                                                       : make_float4(0.f, 0.f, 0.f, 0.f);
-      const float n = fmaxf(m, ml.x), base = n == -INFINITY ? 0.f : n;
-      const float f = exp2_approx(m - base), g = exp2_approx(ml.x - base);
-      m = n;
-      l = l * f + ml.y * g;
-      acc.x = acc.x * f + v.x * g, acc.y = acc.y * f + v.y * g;
-      acc.z = acc.z * f + v.z * g, acc.w = acc.w * f + v.w * g;
+    for (int c = 0; c < count; ++c) {
+      const float f = __shfl_sync(~0u, weight, c);
+      l += f * __shfl_sync(~0u, ml.y, c);
+      if (!__shfl_sync(~0u, static_cast<int>(written), c) || d >= p.dim) continue;
+      const float4 v = *reinterpret_cast<const float4*>(p.part_o + at(c0 + c) * D + d);
+      acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
     }
-    const float inv = seen_by(p, it, query) > 0 ? 1.f / l : 0.f;
-    const int head = kv * p.group + row % p.group;
-    if (d < p.dim)
-      *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (static_cast<int64_t>(it.row0 + query) * p.heads + head) * p.dim + d) =
-          make_uint2(pack16<T>(acc.x * inv, acc.y * inv), pack16<T>(acc.z * inv, acc.w * inv));
   }
+  const float inv = seen_by(p, it, query) > 0 ? 1.f / l : 0.f;
+  const int head = kv * p.group + row % p.group;
+  if (d < p.dim)
+    *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (static_cast<int64_t>(it.row0 + query) * p.heads + head) * p.dim + d) =
+        make_uint2(pack16<T>(acc.x * inv, acc.y * inv), pack16<T>(acc.z * inv, acc.w * inv));
 }
 
 // What depends on the shapes and the hints alone.
@@ -792,7 +869,7 @@ Plan make_plan(const b200q_attention& a) {
 }
 
 template <typename T, int D>
-int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PrefillParams& p, const Plan& plan,
+int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, PrefillParams p, const Plan& plan,
            cudaStream_t stream) {
   constexpr int smem = smem_bytes<D>();
   static_assert(smem <= 227 * 1024 && 2 * smem > kSmSharedBytes, "one CTA an SM: it takes all tensor memory");
@@ -806,13 +883,13 @@ int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, 
     if (e == cudaSuccess && dev < 64) attr_set[dev] = true;
   }
   int launches = 1;
+  p.ctas = static_cast<int>(plan.planned ? std::min<int64_t>(p.sms, plan.units * p.kv_heads) : plan.items * p.kv_heads);
   if (e == cudaSuccess && plan.planned) {
     e = launch_overlapped(MAX_SHARED, attn_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p);
     ++launches;
   }
-  const int64_t ctas = plan.planned ? std::min<int64_t>(p.sms, plan.units * p.kv_heads) : plan.items * p.kv_heads;
   if (e == cudaSuccess)
-    e = launch_overlapped(MAX_SHARED, kern, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), smem, stream, tq, tk, tv, p);
+    e = launch_overlapped(MAX_SHARED, kern, dim3(p.ctas), dim3(kThreads), smem, stream, tq, tk, tv, p);
   if (e == cudaSuccess && plan.split) {
     e = launch_overlapped(MAX_SHARED, attn_prefill_join_kernel<T, D>, dim3(p.sms, kJoinBlocks), dim3(kJoinThreads), 0, stream, p);
     ++launches;
@@ -845,7 +922,7 @@ int launch_attn_prefill(const b200q_attention& a, void* workspace, int* status, 
   p.causal = a.causal;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.status = status;
-  p.split = plan.split, p.sms = sm_count();
+  p.split = plan.split, p.sms = sm_count(), p.most_units = static_cast<int>(plan.units);
   if (plan.planned) {
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     p.header = reinterpret_cast<Header*>(ws);
