@@ -150,6 +150,8 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
   }
   if (mine > 0) atomicAdd(&work, mine);
   __syncthreads();
+  // Items with more than one and a half times an SM's share are cut into shares: a cut costs the writing and reading of
+  // fp32 sums (8 x 128 queries over 2000 keys, 17 tiles at a share of 15: cut 75 us, whole 57).
   int chunk = INT_MAX;
   if (p.split) {
     const unsigned long long share = (work * p.kv_heads + p.sms - 1) / p.sms;
@@ -161,7 +163,7 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
       for (int i = lane; i < items_of(p, it.n); i += 32) {
         set_item(p, it, i);
         const int all = it.hi;
-        it.pieces = all > chunk ? (all + chunk - 1) / chunk : 1;
+        it.pieces = all > chunk && all - chunk > chunk / 2 ? (all + chunk - 1) / chunk : 1;
         const int each = it.pieces > 1 ? all / it.pieces : all, rest = all - each * it.pieces;
         if (pass == 1 && it.pieces > 1) {
           it.slot = atomicAdd(&slots, it.pieces);
