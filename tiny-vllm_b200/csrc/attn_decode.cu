@@ -39,7 +39,9 @@ constexpr int kConsumers = 4;                   // warps, 16 keys of a tile each
 constexpr int kThreads = 32 * (kConsumers + 1);
 constexpr int kRingBytes = 96 * 1024;           // two CTAs an SM
 constexpr int kCtrlBytes = 256;
-constexpr int kMinChunk = 4;                    // tiles
+constexpr int kSegment = 1;                     // what a segment costs beside its tiles (queries, merging, output), in tiles
+constexpr int kMinChunk = 6;                    // the least of a CTA, in tiles
+constexpr int kUncut = 8;                       // tiles up to which a segment is not worth a join
 constexpr float kLazy = 8.f;
 
 struct DecodeParams {
@@ -66,23 +68,30 @@ __device__ __forceinline__ int clipped(int n, const DecodeParams& p) {
 }
 __device__ __forceinline__ int tiles_of(int length) { return max(1, (length + kTile - 1) / kTile); }
 
-// The pieces of a CTA, one after another.  Every thread walks by itself.
+// The pieces of a CTA, one after another.  Every thread walks by itself.  A segment takes kSegment places in the row of all
+// work, then one for each tile; a piece that is cut off before its first tile is none.
 struct Walk {
   int b, seg, from, to, length;   // tiles [from, to) of the segment
-  int64_t left;                   // tiles behind this piece
+  int ahead;                      // length of the next sequence
+  int64_t left;                   // places behind this piece
   __device__ __forceinline__ bool whole() const { return from == 0 && to == tiles_of(length); }
-  __device__ __forceinline__ void cut() {
-    to = static_cast<int>(min(static_cast<int64_t>(tiles_of(length)), from + left));
-    left -= to - from;
+  __device__ __forceinline__ void look_ahead(const DecodeParams& p) { ahead = b + 1 < p.sequences ? p.lengths[b + 1] : 0; }
+  __device__ __forceinline__ bool cut(int at) {      // from this place of the segment on
+    const int end = static_cast<int>(min(static_cast<int64_t>(tiles_of(length) + kSegment), at + left));
+    left -= end - at;
+    from = max(at - kSegment, 0);
+    to = max(end - kSegment, 0);
+    return to > from;
   }
   // the next piece: neighbouring tiles, or, where no segment is cut, every gridDim.x-th segment; false: none
   __device__ __forceinline__ bool next(const DecodeParams& p) {
-    from = 0;
     if (p.split) {
       if (left <= 0) return false;
       if (++seg == p.segments) {
         seg = 0;
-        length = clipped(p.lengths[++b], p);
+        ++b;
+        length = clipped(ahead, p);
+        look_ahead(p);
       }
     } else {
       const int64_t at = static_cast<int64_t>(b) * p.segments + seg + gridDim.x;
@@ -92,8 +101,7 @@ struct Walk {
       length = clipped(p.lengths[b], p);
       left = INT_MAX;
     }
-    cut();
-    return true;
+    return cut(0);
   }
 };
 
@@ -139,7 +147,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
   // Tiles in front of each thread's share of the sequences.
   const int per = (p.sequences + kThreads - 1) / kThreads, b0 = threadIdx.x * per;
   int64_t mine = 0;
-  for (int b = b0; b < min(b0 + per, p.sequences); ++b) mine += tiles_of(clipped(p.lengths[b], p));
+  for (int b = b0; b < min(b0 + per, p.sequences); ++b) mine += tiles_of(clipped(p.lengths[b], p)) + kSegment;
   int64_t upto = mine;
   for (int x = 1; x < 32; x *= 2) {
     const int64_t o = __shfl_up_sync(~0u, upto, x);
@@ -160,18 +168,19 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
     chunk = max((total + gridDim.x - 1) / static_cast<int64_t>(gridDim.x), static_cast<int64_t>(kMinChunk));
     start = blockIdx.x * chunk;
     if (start >= first && start < first + mine * p.segments) {     // one thread
-      int b = b0, tiles;
+      int b = b0, places;
       while (true) {
         s_walk.length = clipped(p.lengths[b], p);
-        tiles = tiles_of(s_walk.length);
-        if (start < first + static_cast<int64_t>(tiles) * p.segments) break;
-        first += static_cast<int64_t>(tiles) * p.segments;
+        places = tiles_of(s_walk.length) + kSegment;
+        if (start < first + static_cast<int64_t>(places) * p.segments) break;
+        first += static_cast<int64_t>(places) * p.segments;
         ++b;
       }
       s_walk.b = b;
-      s_walk.seg = static_cast<int>((start - first) / tiles);
-      s_walk.from = static_cast<int>((start - first) % tiles);
+      s_walk.seg = static_cast<int>((start - first) / places);
+      s_walk.from = static_cast<int>((start - first) % places);
       s_walk.left = min(chunk, total - start);
+      s_walk.look_ahead(p);
     }
   } else if (threadIdx.x == 0) {
     // whole segments, blockIdx.x, blockIdx.x + gridDim.x, ...: `left` counts for one at a time
@@ -190,7 +199,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
   const bool any = w.left > 0;
   __syncthreads();   // comb (the scan) is free
   if (any) {
-    w.cut();
+    w.cut(w.from);      // (never empty: a CTA's places are more than kSegment or reach the row's end)
     int stage = 0;
     uint32_t phase = 0;
     bool go = true;
@@ -198,15 +207,19 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
       // ------------------------------------------------------------------ producer
       bool alive = true;
       const int boxes = kTile / p.box_rows;            // of a tile; a lane holds the page of one box
+      int page = 0, first_pages = -1;                  // of which sequence they are the first ones
       while (go) {
         const int kv = w.seg / p.head_blocks;
         const int32_t* table = p.tables + w.b * p.table_stride;
-        int page = 0, batch = -1;
+        int batch = -1;
+        // a sequence's key heads have the same first pages
+        if (w.from == 0 && w.b == first_pages) batch = 0;
         const int last = w.length == 0 ? w.from : w.to;
         for (int u = w.from; u < last; ++u) {
           // pages of the next 32 boxes at a time
-          if ((u - w.from) * boxes / 32 != batch || batch < 0) {
+          if ((u - w.from) * boxes / 32 != batch) {
             batch = (u - w.from) * boxes / 32;
+            first_pages = u == 0 ? w.b : -1;
             const int64_t pos = static_cast<int64_t>(u) * kTile + lane * p.box_rows;
             if (pos < w.length) {
               page = table[pos / p.page_size];
@@ -246,11 +259,11 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
       // ------------------------------------------------------------------ consumers
       const int gid = lane >> 2, tid = lane & 3;
       bool alive = true;
-      while (go) {
-        const int kv = w.seg / p.head_blocks, head0 = kv * p.group + (w.seg % p.head_blocks) * 8 * NT;
-        const int rows = min(8 * NT, p.group - (w.seg % p.head_blocks) * 8 * NT);
-        // Q^T as the B operand: lane holds dimensions 16 k + 2 tid, + 1, + 8, + 9 of head gid
-        uint32_t qf[NT][D / 16][2];
+      // Q^T as the B operand: lane holds dimensions 16 k + 2 tid, + 1, + 8, + 9 of head gid
+      uint32_t qf[NT][D / 16][2];
+      const auto load_queries = [&](const Walk& w) {
+        const int block = w.seg % p.head_blocks, head0 = w.seg / p.head_blocks * p.group + block * 8 * NT;
+        const int rows = p.group - block * 8 * NT;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           const T* q = static_cast<const T*>(p.q) + w.b * p.q_token + (head0 + 8 * t + gid) * p.q_head;
@@ -262,6 +275,11 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
               qf[t][k][i] = 8 * t + gid < rows && d < p.dim ? *reinterpret_cast<const uint32_t*>(q + d) : 0u;
             }
         }
+      };
+      load_queries(w);
+      while (go) {
+        const int kv = w.seg / p.head_blocks, head0 = kv * p.group + (w.seg % p.head_blocks) * 8 * NT;
+        const int rows = min(8 * NT, p.group - (w.seg % p.head_blocks) * 8 * NT);
         float o[NT][D / 16][4], top[NT][2], sum[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -354,6 +372,10 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
           }
         }
 
+        // ---- the next piece's queries, on their way while this one's results are merged
+        Walk next = w;
+        go = next.next(p);
+        if (go) load_queries(next);
         // ---- the four warps' results of this piece
 #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -407,7 +429,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
           const int64_t behind = tiles_of(w.length) - w.to;      // tiles of the segment in the CTAs behind this one
           p.joins[blockIdx.x] = make_int4(w.b, w.seg, static_cast<int>(blockIdx.x + (behind + chunk - 1) / chunk), 0);
         }
-        go = w.next(p);
+        w = next;
       }
     }
   }
@@ -482,8 +504,8 @@ Plan make_plan(const b200q_attention& a) {
   const int64_t segments = static_cast<int64_t>(a.sequences) * a.kv_heads * plan.head_blocks;
   const int64_t most = (static_cast<int64_t>(a.table_width) * a.page_size + kTile - 1) / kTile;   // tiles of a segment
   const int64_t ctas = sm_count() * 2;
-  plan.split = most > kMinChunk;
-  plan.grid = static_cast<int>(std::min(ctas, plan.split ? segments * ((most + kMinChunk - 1) / kMinChunk) : segments));
+  plan.split = most > kUncut;
+  plan.grid = static_cast<int>(std::min(ctas, plan.split ? segments * ((most + kSegment + kMinChunk - 1) / kMinChunk) : segments));
   if (plan.split) {
     plan.joins = (plan.grid * sizeof(int4) + 255) / 256 * 256;
     plan.ml = (static_cast<size_t>(plan.grid) * 2 * 8 * plan.nt * sizeof(float2) + 255) / 256 * 256;
