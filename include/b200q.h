@@ -466,9 +466,9 @@ int b200q_w8a8_gemm_noalloc(const int8_t* xq, const float* a_scales, const int8_
  *
  * over the keys j that row i sees.  In a sequence with n queries and m keys (0 <= n, m; the queries
  * are the last n of m positions) causal attention shows row i the keys j <= i + m - n; without
- * `causal` every row sees all m.  A row that sees no key gives zeros.  Keys that a row does not see do not
+ * `causal` every row sees all m.  A row that sees no key, or only scores of -infinity, gives zeros.  Keys that a row does not see do not
  * reach it whatever they hold, with one exception: a non-finite value v of a later position of the same sequence
- * may make the rows up to 383 positions before it non-finite, as zero times infinity does in any matrix product.
+ * may make the rows up to 142 positions before it non-finite, as zero times infinity does in any matrix product.
  * Sums and softmax statistics are fp32; the weights exp(s - top) are rounded to T once, as operands of the
  * second product, and the result once.
  *
@@ -503,8 +503,8 @@ typedef struct {
  * Sequences of any lengths, packed one after another (n = 0 and m = 0 included).  Decode: one query
  * per sequence, token b belongs to sequence b, keys and values in pages.  The lengths, tables and
  * pages are read on the device when the kernel runs, so a captured call follows their contents.
- * Lengths are cut to what the tables (packed: key_tokens) hold.  A page outside of the cache counts as zeros and sets the
- * device status word to 0xa01.  workspace: *_workspace_bytes() of the same arguments (0 -> NULL ok);
+ * Lengths are cut to what the tables (packed: key_tokens, tokens) hold.  A page outside of the cache counts as zeros and
+ * sets the device status word to 0xa01; cu_q that does not rise may set it to 0xa03 (and leaves rows unwritten).  workspace: *_workspace_bytes() of the same arguments (0 -> NULL ok);
  * it holds nothing from one call to the next, and calls that overlap need one each.
  */
 int b200q_attn_prefill(const b200q_attention* a, void* workspace, size_t workspace_bytes, void* stream);

@@ -10,10 +10,10 @@ With ``G = heads / kv_heads`` and a sequence of ``n`` queries and ``m`` keys, th
 
     o[i, h] = sum_j p[i, h, j] v[j, h // G],    p = softmax_j(scale * q[i, h] . k[j, h // G])
 
-over ``j <= i + m - n`` (``causal``) or all ``j < m``; zeros where that leaves no key.  Sums and softmax statistics
+over ``j <= i + m - n`` (``causal``) or all ``j < m``; zeros where that leaves no key, or only scores of -infinity.  Sums and softmax statistics
 are fp32; the softmax weights are rounded to the tensors' type for the second product, as is the result.  What
 keys hold that a row does not see does not matter, NaN and infinities included, with one exception: a non-finite
-*value* at a later position of the same sequence may reach rows up to 383 positions before it, as zero times
+*value* at a later position of the same sequence may reach rows up to 142 positions before it, as zero times
 infinity does in any matrix product.
 
 ``float16`` or ``bfloat16``; ``dim`` a multiple of 8 up to 128; up to 128 query heads per key head; pages of a
@@ -111,13 +111,13 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seql
     ``block_tables[b, j // page size]`` (a prompt whose beginning is cached, a chunk of a long one); of
     ``cu_seqlens_k`` only the differences count.  Both ``cu_seqlens`` are int32 ``[sequences + 1]`` on the GPU;
     ``max_seqlen_q`` and ``max_seqlen_k`` bound the lengths and only help to divide the work: the result does not
-    depend on them beyond rounding.  ``scale`` defaults to ``dim ** -0.5``.
+    depend on them beyond rounding.  ``scale`` is positive and defaults to ``dim ** -0.5``.
 
     Returns ``[tokens, heads, dim]`` (``out``, where that is given, contiguous).  Rows behind the last sequence are
     not written.
     """
     if scale is None:
-        scale = q.shape[-1] ** -0.5
+        scale = max(q.shape[-1], 1) ** -0.5
     o = _native().attention(q, k, v, cu_seqlens_q, cu_seqlens_k, None, block_tables, max_seqlen_q, max_seqlen_k, scale,
                             causal, out)
     if o is not None:
@@ -160,13 +160,13 @@ def decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     ``q``: ``[sequences, heads, dim]``; caches ``[pages, page size, kv heads, dim]``; ``context_lens``: int32
     ``[sequences]``, the positions that each token sees, its own among them (0, as in the padding of a captured batch:
     zeros); ``block_tables``: int32 ``[sequences, pages of the longest]``, of which entries behind a sequence's
-    last page are not read.  Lengths are cut to what a row of the tables holds.  ``scale`` defaults to
-    ``dim ** -0.5``.  Returns ``[sequences, heads, dim]`` (``out``, where that is given, contiguous).
+    last page are not read.  Lengths are cut to what a row of the tables holds.  ``scale`` is positive and defaults
+    to ``dim ** -0.5``.  Returns ``[sequences, heads, dim]`` (``out``, where that is given, contiguous).
 
     A long context is divided over the GPU and joined in a fixed order: the same call gives the same bits.
     """
     if scale is None:
-        scale = q.shape[-1] ** -0.5
+        scale = max(q.shape[-1], 1) ** -0.5
     o = _native().attention(q, k_cache, v_cache, None, None, context_lens, block_tables, 1, 0, scale, True, out)
     if o is not None:
         return o

@@ -25,6 +25,12 @@ int check(const b200q_attention* a, bool decode) {
     return B200Q_ERR_UNSUPPORTED_SHAPE;
   for (const b200q_view* x : {&a->q, &a->k, &a->v})
     if (int rc = check_view(*x)) return rc;
+  // a stride of zero would make rows of the same memory, which no TMA descriptor describes
+  if ((a->tokens > 1 && a->q.token == 0) || (a->heads > 1 && a->q.head == 0)) return B200Q_ERR_UNSUPPORTED_SHAPE;
+  for (const b200q_view* x : {&a->k, &a->v})
+    if (((paged ? a->page_size : a->key_tokens) > 1 && x->token == 0) || (a->kv_heads > 1 && x->head == 0) ||
+        (paged && a->pages > 1 && x->page == 0))
+      return B200Q_ERR_UNSUPPORTED_SHAPE;
   for (const void* x : {static_cast<const void*>(a->cu_q), static_cast<const void*>(a->cu_k),
                         static_cast<const void*>(a->lengths), static_cast<const void*>(a->tables)})
     if ((reinterpret_cast<uintptr_t>(x) & 3u) != 0) return B200Q_ERR_MISALIGNED;

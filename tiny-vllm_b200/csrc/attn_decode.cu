@@ -414,7 +414,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
               acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
             }
             if (whole) {
-              const float inv = w.length == 0 ? 0.f : 1.f / l;
+              const float inv = inverse(l);
               uint2 packed = make_uint2(pack16<T>(acc.x * inv, acc.y * inv), pack16<T>(acc.z * inv, acc.w * inv));
               *reinterpret_cast<uint2*>(static_cast<T*>(p.out) +
                                         (static_cast<int64_t>(w.b) * p.heads + head0 + row) * p.dim + d) = packed;
@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const Decode
     l += ml_s[x].y * f;
     acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
   }
-  const float inv = 1.f / l;
+  const float inv = inverse(l);
   const int head = kv * p.group + block * 8 * NT + row;
   *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (static_cast<int64_t>(join.x) * p.heads + head) * p.dim + d) =
       make_uint2(pack16<T>(acc.x * inv, acc.y * inv), pack16<T>(acc.z * inv, acc.w * inv));

@@ -69,28 +69,41 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
+// 1 / sum of weights; 0 where there are none (a row that sees no key, or whose scores are all -inf, gives zeros).
+__device__ __forceinline__ float inverse(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }
+
 // 2^x of two values without the exponential unit: x = n + f with n = round(x) by adding 1.5 2^23, then 2^f on [-1/2, 1/2] by a
 // polynomial of degree 4 with constant term 1 (coefficients fitted for the least largest relative error, 2.9e-6 = 2^-18.4
-// in fp32), and n added to the exponent.  x <= 127.  Below -127 (-inf too) f = 0 and the result is exactly 0.
+// in fp32), times 2^n.  x <= 127.  Below -127 (-inf too) n = -127, whose power comes out as 0; NaN stays NaN.
 __device__ __forceinline__ float2 exp2_poly(uint64_t x) {
   constexpr float kShift = 12582912.f;
-  float2 v = unpair(x);
-  x = pair(fmaxf(v.x, -127.f), fmaxf(v.y, -127.f));
+  const float2 v = unpair(x);
+  x = pair(max_nan(v.x, -127.f), max_nan(v.y, -127.f));
   const uint64_t n = add2(x, pair(kShift, kShift));
   const uint64_t f = fma2(add2(n, pair(-kShift, -kShift)), pair(-1.f, -1.f), x);
   uint64_t y = fma2(f, pair(0.009582852944731712f, 0.009582852944731712f), pair(0.055906426161527634f, 0.055906426161527634f));
   y = fma2(y, f, pair(0.24024099111557007f, 0.24024099111557007f));
   y = fma2(y, f, pair(0.6931241750717163f, 0.6931241750717163f));
   y = fma2(y, f, pair(1.f, 1.f));
-  const float2 m = unpair(n), r = unpair(y);
-  return make_float2(__uint_as_float((__float_as_uint(m.x) << 23) + __float_as_uint(r.x)),
-                     __uint_as_float((__float_as_uint(m.y) << 23) + __float_as_uint(r.y)));
+  const float2 m = unpair(n);
+  return unpair(mul2(y, pair(__uint_as_float((__float_as_uint(m.x) << 23) + 0x3f800000u),
+                             __uint_as_float((__float_as_uint(m.y) << 23) + 0x3f800000u))));
 }
 
 }  // namespace

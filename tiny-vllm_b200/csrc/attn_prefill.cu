@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
           it.hi = it.lo + each + (c < rest);
           const int at = atomicAdd(&count[kBuckets - 1 - min(it.hi - it.lo, kBuckets - 1)], 1);
           if (pass == 1) {
-            p.units[at] = it;
+            if (at < p.most_units) p.units[at] = it;
             ++it.slot;
           }
         }
@@ -201,7 +201,11 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
       __syncthreads();
       if (warp > 0) upto += sums[warp - 1];
       count[threadIdx.x] = upto - own;
-      if (threadIdx.x == kPlanThreads - 1) p.header->units = upto, p.header->next = p.ctas;
+      if (threadIdx.x == kPlanThreads - 1) {
+        // more than sequences that follow one another can have: the list ends where its memory does
+        if (upto > p.most_units) atomicCAS(p.status, 0, 0xa03);
+        p.header->units = min(upto, p.most_units), p.header->next = p.ctas;
+      }
       __syncthreads();
     }
   }
@@ -579,7 +583,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       // rows of one query are neighbours; the next query is all heads further
       uint8_t* base = reinterpret_cast<uint8_t*>(static_cast<T*>(p.out) +
                                                  (static_cast<int64_t>(it.row0 + to) * p.heads + it.kv * p.group) * p.dim);
-      const float inv = 1.f / sum;
+      const float inv = inverse(sum);
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) {
 #pragma unroll
@@ -833,7 +837,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_prefill_join_kernel(const P
       acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
     }
   }
-  const float inv = seen_by(p, it, query) > 0 ? 1.f / l : 0.f;
+  const float inv = inverse(l);
   const int head = kv * p.group + row % p.group;
   if (d < p.dim)
     *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (static_cast<int64_t>(it.row0 + query) * p.heads + head) * p.dim + d) =
