@@ -143,6 +143,7 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
   unsigned long long mine = 0;
   for (int b = p.split ? warp : p.sequences; b < p.sequences; b += 32) {
     Item it = sequence_of(p, cu_q, cu_k, b);
+#pragma unroll 1
     for (int i = lane; i < items_of(p, it.n); i += 32) {
       set_item(p, it, i);
       mine += it.hi;
@@ -153,13 +154,13 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
   // Items with more than one and a half times an SM's share are cut into shares: a cut costs the writing and reading of
   // fp32 sums (8 x 128 queries over 2000 keys, 17 tiles at a share of 15: cut 75 us, whole 57).
   int chunk = INT_MAX;
-  if (p.split) {
-    const unsigned long long share = (work * p.kv_heads + p.sms - 1) / p.sms;
-    chunk = static_cast<int>(min(max(share, static_cast<unsigned long long>(kMinChunk)), static_cast<unsigned long long>(INT_MAX)));
-  }
+  if (p.split)
+    chunk = max(static_cast<int>(min(static_cast<float>(work) * p.kv_heads / p.sms, 1e9f)) + 1, kMinChunk);
+#pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
     for (int b = warp; b < p.sequences; b += 32) {
       Item it = sequence_of(p, cu_q, cu_k, b);
+#pragma unroll 1
       for (int i = lane; i < items_of(p, it.n); i += 32) {
         set_item(p, it, i);
         const int all = it.hi;
@@ -169,6 +170,7 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
           it.slot = atomicAdd(&slots, it.pieces);
           p.joins[atomicAdd(&joins, 1)] = it;
         }
+#pragma unroll 1
         for (int c = 0; c < it.pieces; ++c) {
           it.lo = c * each + min(c, rest);
           it.hi = it.lo + each + (c < rest);
@@ -805,43 +807,44 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
 
 // The pieces of an item that was cut, in their order: a warp takes a row, a lane four dimensions (and the statistics of every 32nd
 // piece).
-constexpr int kJoinThreads = 256, kJoinBlocks = 2 * kRows / (kJoinThreads / 32);
+constexpr int kJoinThreads = 256, kJoinBlocks = 8;      // blocks an SM: one wave, which ends at once where nothing was cut
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) attn_prefill_join_kernel(const PrefillParams p) {
   ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
-  if (static_cast<int>(blockIdx.x) >= p.header->joins * p.kv_heads) return;
-  const Item it = p.joins[blockIdx.x / p.kv_heads];
-  const int kv = blockIdx.x % p.kv_heads, lane = threadIdx.x & 31, d = lane * 4;
-  const int r = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5), row = r % kRows;
-  const int query = it.first + r / kRows * p.tile_tokens + row / p.group;
-  if (row >= p.tile_tokens * p.group || query >= it.n) return;
-  const auto at = [&](int c) { return (static_cast<int64_t>(it.slot + c) * p.kv_heads + kv) * 2 * kRows + r; };
-  float top = -INFINITY;
-  for (int c = lane; c < it.pieces; c += 32) top = fmaxf(top, p.part_ml[at(c)].x);
-  for (int x = 16; x > 0; x /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
-  const float base = top == -INFINITY ? 0.f : top;
-  float l = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int c0 = 0; c0 < it.pieces; c0 += 32) {
-    const float2 ml = c0 + lane < it.pieces ? p.part_ml[at(c0 + lane)] : make_float2(-INFINITY, 0.f);
-    const float weight = exp2_approx(ml.x - base);
-    const bool written = ml.x != -INFINITY;      // a piece of which the row's tile sees nothing has written no sums
-    const int count = min(it.pieces - c0, 32);
+  const int lane = threadIdx.x & 31, d = lane * 4, rows = p.header->joins * p.kv_heads * 2 * kRows;
+  for (int all = blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5); all < rows; all += gridDim.x * (kJoinThreads / 32)) {
+    const int r = all % (2 * kRows), row = r % kRows, kv = all / (2 * kRows) % p.kv_heads;
+    const Item& it = p.joins[all / (2 * kRows) / p.kv_heads];
+    const int query = it.first + r / kRows * p.tile_tokens + row / p.group;
+    if (row >= p.tile_tokens * p.group || query >= it.n) continue;
+    const auto at = [&](int c) { return (static_cast<int64_t>(it.slot + c) * p.kv_heads + kv) * 2 * kRows + r; };
+    float top = -INFINITY;
+    for (int c = lane; c < it.pieces; c += 32) top = fmaxf(top, p.part_ml[at(c)].x);
+    for (int x = 16; x > 0; x /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
+    const float base = top == -INFINITY ? 0.f : top;
+    float l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c0 = 0; c0 < it.pieces; c0 += 32) {
+      const float2 ml = c0 + lane < it.pieces ? p.part_ml[at(c0 + lane)] : make_float2(-INFINITY, 0.f);
+      const float weight = exp2_approx(ml.x - base);
+      const bool written = ml.x != -INFINITY;      // a piece of which the row's tile sees nothing has written no sums
+      const int count = min(it.pieces - c0, 32);
 #pragma unroll 4
-    for (int c = 0; c < count; ++c) {
-      const float f = __shfl_sync(~0u, weight, c);
-      l += f * __shfl_sync(~0u, ml.y, c);
-      if (!__shfl_sync(~0u, static_cast<int>(written), c) || d >= p.dim) continue;
-      const float4 v = *reinterpret_cast<const float4*>(p.part_o + at(c0 + c) * D + d);
-      acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+      for (int c = 0; c < count; ++c) {
+        const float f = __shfl_sync(~0u, weight, c);
+        l += f * __shfl_sync(~0u, ml.y, c);
+        if (!__shfl_sync(~0u, static_cast<int>(written), c) || d >= p.dim) continue;
+        const float4 v = *reinterpret_cast<const float4*>(p.part_o + at(c0 + c) * D + d);
+        acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+      }
     }
+    const float inv = inverse(l);
+    const int head = kv * p.group + row % p.group;
+    if (d < p.dim)
+      *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (static_cast<int64_t>(it.row0 + query) * p.heads + head) * p.dim + d) =
+          make_uint2(pack16<T>(acc.x * inv, acc.y * inv), pack16<T>(acc.z * inv, acc.w * inv));
   }
-  const float inv = inverse(l);
-  const int head = kv * p.group + row % p.group;
-  if (d < p.dim)
-    *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (static_cast<int64_t>(it.row0 + query) * p.heads + head) * p.dim + d) =
-        make_uint2(pack16<T>(acc.x * inv, acc.y * inv), pack16<T>(acc.z * inv, acc.w * inv));
 }
 
 // What depends on the shapes and the hints alone.
@@ -859,9 +862,9 @@ Plan make_plan(const b200q_attention& a) {
   // at most one item of each sequence is not full
   plan.items = std::min<int64_t>(a.tokens, a.tokens / plan.per_item + static_cast<int64_t>(a.sequences));
   // No item is cut where the longest has no more than an SM's share of all keys, each item having one tile of keys at
-  // least; nor where it is short.
+  // least; nor where it is short (64 queries over 2000 keys: whole 31 us, cut and joined 30; over 1100: 20 and 29).
   const int64_t longest = (static_cast<int64_t>(a.max_k) + kRows - 1) / kRows;
-  plan.split = longest > kMinChunk && a.tokens / plan.per_item * a.kv_heads < sms * longest;
+  plan.split = longest > 2 * kMinChunk && a.tokens / plan.per_item * a.kv_heads < sms * longest;
   plan.planned = plan.split || plan.items * a.kv_heads > sms;
   plan.units = plan.items + (plan.split ? 2 * sms : 0);
   if (!plan.planned) return plan;
@@ -897,7 +900,7 @@ int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, 
   if (e == cudaSuccess)
     e = launch_overlapped(MAX_SHARED, kern, dim3(p.ctas), dim3(kThreads), smem, stream, tq, tk, tv, p);
   if (e == cudaSuccess && plan.split) {
-    e = launch_overlapped(MAX_SHARED, attn_prefill_join_kernel<T, D>, dim3(p.sms, kJoinBlocks), dim3(kJoinThreads), 0, stream, p);
+    e = launch_overlapped(MAX_SHARED, attn_prefill_join_kernel<T, D>, dim3(p.sms * kJoinBlocks), dim3(kJoinThreads), 0, stream, p);
     ++launches;
   }
   if (e != cudaSuccess) {
