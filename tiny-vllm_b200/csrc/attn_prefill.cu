@@ -828,15 +828,21 @@ __global__ void __launch_bounds__(kJoinThreads) attn_prefill_join_kernel(const P
     for (int c0 = 0; c0 < it.pieces; c0 += 32) {
       const float2 ml = c0 + lane < it.pieces ? p.part_ml[at(c0 + lane)] : make_float2(-INFINITY, 0.f);
       const float weight = exp2_approx(ml.x - base);
-      const bool written = ml.x != -INFINITY;      // a piece of which the row's tile sees nothing has written no sums
       const int count = min(it.pieces - c0, 32);
-#pragma unroll 4
-      for (int c = 0; c < count; ++c) {
-        const float f = __shfl_sync(~0u, weight, c);
-        l += f * __shfl_sync(~0u, ml.y, c);
-        if (!__shfl_sync(~0u, static_cast<int>(written), c) || d >= p.dim) continue;
-        const float4 v = *reinterpret_cast<const float4*>(p.part_o + at(c0 + c) * D + d);
-        acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+      for (int c1 = 0; c1 < count; c1 += 8) {
+        float4 v[8];      // all on their way at once
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          v[i] = c1 + i < count && d < p.dim ? *reinterpret_cast<const float4*>(p.part_o + at(c0 + c1 + i) * D + d)
+                                             : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int c = min(c1 + i, 31);
+          const float f = __shfl_sync(~0u, weight, c), m = __shfl_sync(~0u, ml.x, c), s = __shfl_sync(~0u, ml.y, c);
+          if (c1 + i >= count || m == -INFINITY) continue;      // a piece of which the row sees nothing: its sums may be anything
+          l += f * s;
+          acc.x += v[i].x * f, acc.y += v[i].y * f, acc.z += v[i].z * f, acc.w += v[i].w * f;
+        }
       }
     }
     const float inv = inverse(l);
