@@ -14,13 +14,15 @@
 //   S_t = Q_t K^T    both operands in shared memory
 //   O_t += P_t V      P from tensor memory, V as rows of keys
 // Keys go from the last tile, where the mask is, to the first.  The running maximum is raised, and O_t rescaled in place, only
-// when a score exceeds it by more than 8 (weights reach 2^8 at most, rounded with the same relative error).
+// when a score exceeded it by more than 8 in the step before, or does so by more than 14 now (weights reach 2^14 at most,
+// rounded with the same relative error).
 //
 // Work: an item is two tiles of queries and their keys.  Where there are more items than SMs, or one of them might be long, a
 // small kernel (attn_plan_kernel) lists them first, those with the most keys at the front, and CTAs, one an SM, take one
-// after another; the next item's Q and K arrive, and its first scores are formed, under the last exponentials and the output
-// of the one before.  An item with more than an SM's share of all keys is cut into pieces, which leave fp32 partial
-// results for a third kernel to join in their order: few queries over a long cached prefix then use the whole GPU.
+// after another; the next item's Q and K arrive under the last exponentials of the one before, whose output stands behind the
+// first exponentials of the next.  An item with more than one and a half times an SM's share of all keys is cut into
+// pieces, which leave fp32 partial results for a third kernel to join in their order: few queries over a long cached prefix
+// then use the whole GPU.
 //
 // Warps: 0-3 and 4-7 softmax of tile 0 and 1, a row a thread; 8 issues the products; 9 brings Q, K and V; 10 fetches
 // items; 11 clears the end of a sequence's last V tile.
@@ -769,7 +771,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
 #pragma unroll
         for (int i = 0; i < 4; ++i) most[i] = -INFINITY;
         weights(0, 32);
-        want = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * p.scale_log2;
+        want = limit > 0 ? fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * p.scale_log2 : -INFINITY;
         if (__any_sync(~0u, want > top + kMost)) {
           raise(fmaxf(want, top));
           part[0] = part[1] = pair(0.f, 0.f);
