@@ -525,7 +525,7 @@ int b200q_kv_store(const b200q_view* k, const b200q_view* v, const b200q_view* k
 /*
  * Copies whole pages: page src[i] to page dst[i], in each of `outer` caches (layers, keys and values) that
  * begin outer_stride bytes apart and whose dense pages of page_bytes begin page_stride bytes apart (all
- * multiples of 16).  src and dst are HOST arrays, read before the call returns (a captured call keeps its pairs).
+ * multiples of 16; pages do not overlap).  src and dst are HOST arrays, read before the call returns (a captured call keeps its pairs).
  * A page may be copied to several places; a destination stands once, and no page is source and destination
  * of one call (B200Q_ERR_BAD_ARGUMENT, as for a page outside of the cache).  No counterpart in the reference.
  */

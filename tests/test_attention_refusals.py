@@ -171,7 +171,8 @@ ARGUMENTS = [
     ({"out": None}, _lib.ERR_NULL_POINTER), ({"data_of_k": None}, _lib.ERR_NULL_POINTER), ({"tables": None}, _lib.ERR_NULL_POINTER),
     ({"dtype": 7}, _lib.ERR_BAD_ARGUMENT), ({"scale": float("nan")}, _lib.ERR_BAD_ARGUMENT), ({"scale": 0.0}, _lib.ERR_BAD_ARGUMENT),
     ({"scale": float("inf")}, _lib.ERR_BAD_ARGUMENT), ({"scale": -1.0}, _lib.ERR_BAD_ARGUMENT),
-    ({"tokens": 0}, _lib.ERR_BAD_SHAPE), ({"sequences": 0}, _lib.ERR_BAD_SHAPE), ({"heads": 3}, _lib.ERR_BAD_SHAPE),
+    ({"tokens": 0}, _lib.ERR_BAD_SHAPE), ({"tokens": 2 ** 31 - 1}, _lib.ERR_BAD_SHAPE),
+    ({"page_size": 0, "key_tokens": 2 ** 31 - 1}, _lib.ERR_BAD_SHAPE), ({"sequences": 0}, _lib.ERR_BAD_SHAPE), ({"heads": 3}, _lib.ERR_BAD_SHAPE),
     ({"kv_heads": 0}, _lib.ERR_BAD_SHAPE), ({"pages": 0}, _lib.ERR_BAD_SHAPE), ({"table_width": 0}, _lib.ERR_BAD_SHAPE),
     ({"page_size": -16}, _lib.ERR_BAD_SHAPE), ({"max_k": -1}, _lib.ERR_BAD_SHAPE), ({"heads": 1 << 16}, _lib.ERR_BAD_SHAPE),
     ({"dim": 60}, _lib.ERR_UNSUPPORTED_SHAPE), ({"dim": 136}, _lib.ERR_UNSUPPORTED_SHAPE), ({"heads": 258}, _lib.ERR_UNSUPPORTED_SHAPE),
@@ -221,7 +222,7 @@ def test_store_and_copy_check_their_arguments(L):
 
     assert stored(slots=None) == _lib.ERR_NULL_POINTER
     assert stored(c=_lib.View(None, 0, 0, 0)) == _lib.ERR_NULL_POINTER
-    assert stored(tokens=0) == stored(pages=0) == stored(size=0) == _lib.ERR_BAD_SHAPE
+    assert stored(tokens=0) == stored(tokens=2 ** 31 - 1) == stored(pages=0) == stored(size=0) == _lib.ERR_BAD_SHAPE
     assert stored(dim=60) == stored(k=_lib.View(p, 0, 100, 64)) == _lib.ERR_UNSUPPORTED_SHAPE
     assert stored(k=_lib.View(p + 8, 0, 128, 64)) == stored(slots=p + 2) == _lib.ERR_MISALIGNED
 
@@ -235,7 +236,8 @@ def test_store_and_copy_check_their_arguments(L):
     assert copied(cache=p + 8) == _lib.ERR_MISALIGNED
     for src, dst in (((0,), (5,)), ((-1,), (1,)), ((0, 1), (2, 2)), ((0, 1), (2, 0)), ((4,), (4,))):
         assert copied(src, dst) == _lib.ERR_BAD_ARGUMENT
-    assert copied((0, 0), (1, 2)) in (_lib.ERR_LAUNCH, _lib.ERR_UNSUPPORTED_ARCH, _lib.OK)
+    # pages or layers that overlap
+    assert copied(page_stride=0) == copied(page_stride=4080) == copied(outer_stride=0) == _lib.ERR_UNSUPPORTED_SHAPE
 
 
 def test_structures_are_the_headers(tmp_path):

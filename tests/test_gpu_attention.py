@@ -172,6 +172,27 @@ def test_large_scores():
         check(got, want[-1:], tol[-1:])
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_the_largest_scores(dtype):
+    # q . k = 2^24 for one key of each row's, at most 2^23 for the others: a row is that key's value
+    n, dim = 300, 64
+    one = torch.zeros(n, 1, dim, dtype=dtype, device="cuda")
+    one[:, 0, 0] = 4096
+    k = one / torch.arange(2, n + 2, device="cuda", dtype=torch.float32)[:, None, None].to(dtype)
+    for best in (0, 7, 150, 299):
+        kk = k.clone()
+        kk[best] = one[best]
+        v = rows(generator(best), n, 1, dim, dtype)
+        got = prefill_attention(one, kk, v, cumulated([n]), cumulated([n]), n, n, scale=1.0)
+        # the weight, whose 32-bit argument may be off by one, is rounded to the type; its sum is not; then the result is
+        want = v[best:best + 1].double().expand(n - best, 1, dim)
+        check(got[best:], want, (torch.finfo(dtype).eps + 2.0 ** -15) * want.abs() + 2.0 ** -24)
+        paged = Paged(generator(1), kk, v, [n], 16)
+        got = decode_attention(one[-1:], paged.k, paged.v, torch.tensor([n], dtype=torch.int32, device="cuda"), paged.tables,
+                               scale=1.0)
+        assert torch.equal(got, v[best:best + 1])
+
+
 def test_infinite_and_lowest_scores():
     # a key at the type's lowest value (its scores are -inf or of the order of the largest float), one of zeros
     q = torch.ones(3, 2, 64, dtype=BF, device="cuda")

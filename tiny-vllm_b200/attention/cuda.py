@@ -14,7 +14,8 @@ over ``j <= i + m - n`` (``causal``) or all ``j < m``; zeros where that leaves n
 are fp32; the softmax weights are rounded to the tensors' type for the second product, as is the result.  What
 keys hold that a row does not see does not matter, NaN and infinities included, with one exception: a non-finite
 *value* at a later position of the same sequence may reach rows up to 142 positions before it, as zero times
-infinity does in any matrix product.
+infinity does in any matrix product.  Scores ``scale * q . k`` are fp32 and may reach 2^24 in magnitude, from where on
+fp32 does not tell neighbours apart; rows of prompts with larger ones may be wrong.
 
 ``float16`` or ``bfloat16``; ``dim`` a multiple of 8 up to 128; up to 128 query heads per key head; pages of a
 multiple of 16 positions.  Heads, tokens and pages may stand apart (strides of a multiple of 8 elements).  Calls run on

@@ -17,6 +17,7 @@ int check(const b200q_attention* a, bool decode) {
   if (!(a->scale > 0) || !(a->scale < 1e38f)) return B200Q_ERR_BAD_ARGUMENT;
   if (a->tokens <= 0 || a->sequences <= 0 || a->heads <= 0 || a->kv_heads <= 0 || a->dim <= 0 || a->max_q < 0 || a->max_k < 0)
     return B200Q_ERR_BAD_SHAPE;
+  if (a->tokens > kMostTokens || a->key_tokens > kMostTokens) return B200Q_ERR_BAD_SHAPE;
   if (decode && (!paged || a->tokens != a->sequences)) return B200Q_ERR_BAD_SHAPE;
   if (paged ? a->pages <= 0 || a->page_size < 0 || a->table_width <= 0 || a->table_stride < 0 : a->key_tokens < 0)
     return B200Q_ERR_BAD_SHAPE;
@@ -65,7 +66,7 @@ int b200q_attn_decode(const b200q_attention* a, void* workspace, size_t workspac
   return run(a, true, workspace, workspace_bytes, stream);
 }
 
-size_t b200q_attn_prefill_workspace_bytes(const b200q_attention* a) { 
+size_t b200q_attn_prefill_workspace_bytes(const b200q_attention* a) {
   return check(a, false) == B200Q_OK ? attn_prefill_workspace(*a) : 0;
 }
 size_t b200q_attn_decode_workspace_bytes(const b200q_attention* a) {

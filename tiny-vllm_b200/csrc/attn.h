@@ -9,6 +9,9 @@
 
 namespace b200q {
 
+// Tokens of a call: a tile beyond stays within 32 bits.
+constexpr int kMostTokens = 0x7fffffff - 1024;
+
 // b200q_view's rules.
 inline int check_view(const b200q_view& x) {
   if (x.data == nullptr) return B200Q_ERR_NULL_POINTER;

@@ -107,7 +107,7 @@ __device__ __forceinline__ int items_of(const PrefillParams& p, int n) {
 }
 // Keys that query i sees: [0, seen).
 __device__ __forceinline__ int seen_by(const PrefillParams& p, const Item& it, int i) {
-  return max(0, p.causal ? min(it.m, i + 1 + it.m - it.n) : it.m);
+  return max(0, p.causal ? min(it.m, it.m - it.n + i + 1) : it.m);
 }
 __device__ __forceinline__ Item sequence_of(const PrefillParams& p, const int* cu_q, const int* cu_k, int b) {
   Item it{};

@@ -103,7 +103,8 @@ extern "C" int b200q_kv_store(const b200q_view* k, const b200q_view* v, const b2
                               int pages, int page_size, void* stream) {
   if (k == nullptr || v == nullptr || k_cache == nullptr || v_cache == nullptr || slots == nullptr)
     return B200Q_ERR_NULL_POINTER;
-  if (tokens <= 0 || kv_heads <= 0 || dim <= 0 || pages <= 0 || page_size <= 0) return B200Q_ERR_BAD_SHAPE;
+  if (tokens <= 0 || kv_heads <= 0 || dim <= 0 || pages <= 0 || page_size <= 0 || tokens > kMostTokens)
+    return B200Q_ERR_BAD_SHAPE;
   if (static_cast<int64_t>(kv_heads) * dim > INT_MAX) return B200Q_ERR_BAD_SHAPE;
   if ((dim % 8) != 0) return B200Q_ERR_UNSUPPORTED_SHAPE;
   for (const b200q_view* x : {k, v, k_cache, v_cache})
@@ -137,7 +138,7 @@ extern "C" int b200q_kv_copy_pages(void* cache, int64_t outer, int64_t outer_str
   if (outer <= 0 || outer > 65535 || page_bytes <= 0 || pages <= 0 || count <= 0) return B200Q_ERR_BAD_SHAPE;
   if (page_bytes / 16 > static_cast<int64_t>(INT_MAX) * kCopyThreads) return B200Q_ERR_BAD_SHAPE;
   if ((page_bytes % 16) != 0 || (page_stride % 16) != 0 || (outer_stride % 16) != 0 || page_stride < 0 ||
-      outer_stride < 0)
+      outer_stride < 0 || (pages > 1 && page_stride < page_bytes) || (outer > 1 && outer_stride < page_bytes))
     return B200Q_ERR_UNSUPPORTED_SHAPE;
   if ((reinterpret_cast<uintptr_t>(cache) & 15u) != 0) return B200Q_ERR_MISALIGNED;
   // bit 0: a source, bit 1: a destination
