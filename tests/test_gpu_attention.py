@@ -172,6 +172,27 @@ def test_large_scores():
         check(got, want[-1:], tol[-1:])
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("gap", [9.0, 90.0, 128.0, 200.0, 1000.0])
+def test_one_key_far_ahead_wherever_it_stands(gap, dim):
+    # 256 sequences of 300 keys: in sequence j key j has a score that is `gap` (of the exponent of 2) above all others
+    n, m = 256, 300
+    q = torch.zeros(n, 2, dim, dtype=BF, device="cuda")
+    q[:, :, 0] = 8.0
+    gen = generator(9)
+    k, v = rows(gen, n * m, 1, dim, BF), rows(gen, n * m, 1, dim, BF)
+    k[:, :, 0] = 0
+    j = torch.arange(n, device="cuda")
+    k[j * m + j, :, 0] = gap / 8
+    keys = [m] * n
+    scale = 0.6931471805599453
+    want, tol = packed_reference(q, k, v, [1] * n, keys, scale)
+    check(prefill_attention(q, k, v, cumulated([1] * n), cumulated(keys), 1, m, scale=scale), want, tol)
+    paged = Paged(gen, k, v, keys, 16)
+    check(decode_attention(q, paged.k, paged.v, torch.tensor(keys, dtype=torch.int32, device="cuda"), paged.tables, scale=scale),
+          want, tol)
+
+
 @pytest.mark.parametrize("dtype", [BF, HF])
 def test_the_largest_scores(dtype):
     # q . k = 2^24 for one key of each row's, at most 2^23 for the others: a row is that key's value

@@ -13,9 +13,9 @@
 // O0, O1 (128 x D sums).  Shared memory: both Q tiles and a ring of K and V tiles.
 //   S_t = Q_t K^T    both operands in shared memory
 //   O_t += P_t V      P from tensor memory, V as rows of keys
-// Keys go from the last tile, where the mask is, to the first.  The running maximum is raised, and O_t rescaled in place, only
-// when a score exceeded it by more than 8 in the step before, or does so by more than 14 now (weights reach 2^14 at most,
-// rounded with the same relative error).
+// Keys go from the last tile, where the mask is, to the first.  `top` is the maximum of a row's first step.  Later steps do not
+// look for theirs: as long as the sum of their weights stays small, `top` may stay as well; else it is raised, and O_t
+// rescaled in place.  Weights reach 2^12 at most, rounded with the same relative error.
 //
 // Work: an item is two tiles of queries and their keys.  Where there are more items than SMs, or one of them might be long, a
 // small kernel (attn_plan_kernel) lists them first, those with the most keys at the front, and CTAs, one an SM, take one
@@ -50,9 +50,10 @@ static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * 168, "register
 constexpr int kCtrlBytes = 1024;
 constexpr int kTmemCols = 512;
 constexpr uint32_t kColO = 256;
-constexpr float kLazy = 8.f, kMost = 14.f;        // log2 of a weight: from where the maximum follows, and the largest
+constexpr float kMost = 4096.f, kMostLog2 = 12.f;  // the largest weight
 constexpr int kMinChunk = 8;                      // tiles of keys: the shortest piece that an item is cut into
 constexpr int kFirstGroups = 6;                   // of 16 keys, whose weights are announced first
+constexpr int kChecked = 48;                      // pairs of weights whose sum says whether the maximum follows
 constexpr int kReaders = 11;                      // warps that read an item
 constexpr int kItems = 4;                         // places for items that are on their way or worked on
 constexpr int kSignals = 8;                       // more than the products can be ahead of the copies: stages / 2 + 1
@@ -612,9 +613,9 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     uint32_t x[kRows], e16[kRows / 2];
     uint64_t part[2];
     float top = 0.f, most[4];
-    // Weights of pairs [from, to), eight at a time; sums, maxima (of all scores, by pair 32) and conversions of eight stand
-    // beside the exponentials of the next.  The exponential unit gives 16 results a cycle for the SM; every fourth pair
-    // goes through the multipliers instead (8192 tokens: no pair 489 us, every 8th 483, every 4th 473, every 2nd 496).
+    // Weights of pairs [from, to), eight at a time; sums, conversions and maxima (of the scores behind kChecked) of eight
+    // stand beside the exponentials of the next.  The exponential unit gives 16 results a cycle for the SM; every eighth pair
+    // goes through the multipliers instead (8 x 1024 tokens: every 4th 96 us, every 8th 93).
     const auto weights = [&](int from, int to) {
       const float base = top == -INFINITY ? 0.f : -top;
       const uint64_t base2 = pair(base, base);
@@ -628,7 +629,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             arg[i] = fma2(pair(__uint_as_float(x[16 * b + 2 * i]), __uint_as_float(x[16 * b + 2 * i + 1])), scale2, base2);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            if (i % 4 == 3) {
+            if (i % 8 == 7) {
               e[b & 1][i] = exp2_poly(arg[i]);
             } else {
               const float2 v = unpair(arg[i]);
@@ -643,10 +644,13 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             const float2 v = e[(b - 1) & 1][i];
             part[i & 1] = add2(part[i & 1], pair(v.x, v.y));
             e16[at] = pack16<T>(v.x, v.y);
-            if (at < 32) {
-              most[i & 1] = max3(most[i & 1], __uint_as_float(x[2 * at]), __uint_as_float(x[2 * at + 1]));
-              most[2 + (i & 1)] = max3(most[2 + (i & 1)], __uint_as_float(x[64 + 2 * at]), __uint_as_float(x[64 + 2 * at + 1]));
+            // (the maximum of the scores whose weights a sum does not check: those behind kChecked and, as exp2_poly is not
+            // for arguments above 127, its own)
+            if (at < kChecked && at % 3 == 0) {
+              const int c = 2 * kChecked + 2 * (at / 3);
+              most[i & 3] = max3(most[i & 3], __uint_as_float(x[c]), __uint_as_float(x[c + 1]));
             }
+            if (at < kChecked && i % 8 == 7) most[i & 3] = max3(most[i & 3], __uint_as_float(x[2 * at]), __uint_as_float(x[2 * at + 1]));
           }
         }
       }
@@ -684,7 +688,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
 #pragma unroll
         for (int i = 0; i < 32; ++i) x[32 * c + i] = (sees >> i) & 1u ? x[32 * c + i] : __float_as_uint(-INFINITY);
       };
-      float sum = 0.f, want = -INFINITY;
+      float sum = 0.f;
       top = -INFINITY;
       if (any) {
         // ---- first step: the maximum comes first
@@ -708,7 +712,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
           for (int i = 0; i < 4; ++i) most[i] = max3(most[i], __uint_as_float(x[c + 2 * i]), __uint_as_float(x[c + 2 * i + 1]));
 #pragma unroll
         for (int i = 0; i < 4; ++i) most[i] = fmaxf(most[i], __uint_as_float(x[kRows - 4 + i]));
-        top = want = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * p.scale_log2;
+        top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * p.scale_log2;
         part[0] = part[1] = pair(0.f, 0.f);
         weights(0, 32);
         ptx::tmem_st_32x32b_x32(col_s, *reinterpret_cast<uint32_t(*)[32]>(e16));
@@ -764,28 +768,33 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             ptx::tmem_st_32x32b_x16(col_o + 16 * c, o);
           }
         };
-        if (__any_sync(~0u, want > top + kLazy)) raise(fmaxf(want, top));
-        // The maximum of these scores is not waited for: it is found beside the exponentials of the first half, and counts
-        // from the next step on.  Only where it is out of reach (weights above 2^14) is the half done again.
         part[0] = part[1] = pair(0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < 4; ++i) most[i] = -INFINITY;
-        weights(0, 32);
-        want = limit > 0 ? fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * p.scale_log2 : -INFINITY;
-        if (__any_sync(~0u, want > top + kMost)) {
-          raise(fmaxf(want, top));
-          part[0] = part[1] = pair(0.f, 0.f);
+        weights(0, 48);
+        // Where the sum of these weights, or the largest of the other scores, is out of reach they are done again.  (Maxima of
+        // all scores instead, found beside the exponentials: 8192 tokens 463 us for 442.)
+        const auto over = [&] {
+          const float2 both = unpair(add2(part[0], part[1]));
+          const float last = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * p.scale_log2;
+          return both.x + both.y > kMost || last > top + kMostLog2 || top == -INFINITY;
+        };
+        if (__any_sync(~0u, over() && limit > begin)) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            load(c);
-            ptx::tmem_ld_wait();
-            if (masked) mask(c, begin);
+          for (int c = 0; c < kChecked / 16; ++c) load(c);
+          ptx::tmem_ld_wait();
+          if (masked) {
+#pragma unroll
+            for (int c = 0; c < kChecked / 16; ++c) mask(c, begin);
           }
-          weights(0, 32);
+#pragma unroll
+          for (int i = 0; i < 2 * kChecked; i += 2) most[i & 2] = max3(most[i & 2], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+          const float to = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * p.scale_log2;
+          raise(limit > begin ? fmaxf(to, top) : top);
+          part[0] = part[1] = pair(0.f, 0.f);
+          weights(0, kChecked);
         }
         ptx::tmem_st_32x32b_x32(col_s, *reinterpret_cast<uint32_t(*)[32]>(e16));
-        // three quarters of the keys first: what is left of the product is then short when the last weights come
-        weights(32, 48);
         ptx::tmem_st_32x32b_x16(col_s + 32, *reinterpret_cast<uint32_t(*)[16]>(e16 + 32));
         announce(0);
         weights(48, 64);
