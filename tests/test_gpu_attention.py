@@ -93,6 +93,25 @@ def test_rows_that_see_nothing_and_empty_sequences(page):
     assert torch.equal(got[:140], torch.zeros_like(got[:140])) and torch.equal(got[200:205], torch.zeros_like(got[:5]))
 
 
+@pytest.mark.parametrize("dim,kv", [(128, 8), (64, 2)])
+def test_many_short_sequences(dim, kv):
+    # items of one tile of keys, whose end is cleared, follow one another as fast as their copies come from memory
+    n, m = 4096, 100
+    gen = generator(22)
+    q, k, v = rows(gen, n, 4 * kv, dim, BF), rows(gen, n * m, kv, dim, BF), rows(gen, n * m, kv, dim, BF)
+    queries, keys = cumulated([1] * n), cumulated([m] * n)
+    got = [prefill_attention(q, k, v, queries, keys, 1, m) for _ in range(10)]
+    qd, kd, vd = (t.double().unflatten(0, (n, -1)) for t in (q, k, v))
+    p = torch.einsum("nxhgd,nmhd->nhgm", qd.unflatten(2, (kv, 4)), kd).mul(dim ** -0.5).softmax(-1)
+    want = torch.einsum("nhgm,nmhd->nhgd", p, vd).flatten(1, 2)
+    # u |o| + (u + 2 (ds + 2^-16) + m 2^-23) A with |o| <= A = sum p |v|, scores under 8: ds < 2^-13
+    tol = (2 * 2.0 ** -8 + 2.0 ** -11) * torch.einsum("nhgm,nmhd->nhgd", p, vd.abs()).flatten(1, 2) + 2.0 ** -26
+    check(got[0], want, tol)
+    for other in got[1:]:
+        assert torch.equal(got[0], other)
+    assert device_status_ok()
+
+
 def test_no_keys_at_all():
     q = torch.ones(7, 4, 128, dtype=BF, device="cuda")
     k = torch.empty(0, 2, 128, dtype=BF, device="cuda")

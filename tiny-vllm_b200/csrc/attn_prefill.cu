@@ -241,13 +241,13 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
   uint64_t* p_bar = s_bar + 2;                              // [2][2] its weights are, of the first keys and the others
   uint64_t* o_bar = p_bar + 4;                              // [2] all products of an item are done
   uint64_t* q_bar = o_bar + 2;
-  uint64_t* tail_bar = q_bar + 1;                           // a last V tile, before its end is cleared
-  uint64_t* want_bar = tail_bar + 1;                        // the next item is wanted
+  uint64_t* tail_bar = q_bar + 1;                           // [stages] a last V tile, before its end is cleared
+  uint64_t* want_bar = tail_bar + kStages;                  // the next item is wanted
   uint64_t* item_bar = want_bar + 1;                        // [items] an item is there
   uint64_t* read_bar = item_bar + kItems;                   // [items] all have read it
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(read_bar + kItems);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert(kItems * sizeof(Item) + 8 * (kStages + kSignals + 11 + 2 * kItems) + 8 <= kCtrlBytes, "control words");
+  static_assert(kItems * sizeof(Item) + 8 * (2 * kStages + kSignals + 10 + 2 * kItems) + 8 <= kCtrlBytes, "control words");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t smem_base = ptx::smem_u32(smem), ring_base = smem_base + 2 * kTileBytes;
@@ -269,7 +269,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       ptx::mbar_init(ptx::smem_u32(read_bar + k), kReaders);
     }
     ptx::mbar_init(ptx::smem_u32(q_bar), 1);
-    ptx::mbar_init(ptx::smem_u32(tail_bar), 1);
+    for (int s = 0; s < kStages; ++s) ptx::mbar_init(ptx::smem_u32(tail_bar + s), 1);
     ptx::mbar_init(ptx::smem_u32(want_bar), 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
@@ -367,7 +367,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     const int boxes = kRows / p.box_rows;
     int stage = 0, freed = 0, signal = 0, q_free = -1;
     int holder = -1;      // lane l: the signal that frees place l of the ring
-    uint32_t phase = 0, tails = 0, queries = 0;
+    uint32_t phase = 0, tails = 0, tail_phase = 0, queries = 0;      // tails, tail_phase: a bit for each place of the ring
     const auto wait_for = [&](int event) {
       for (; freed <= event; ++freed)
         if (alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(free_bar + (freed & (kSignals - 1))), (freed / kSignals) & 1, abort_flag));
@@ -418,14 +418,17 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         for (int x = 0; x < 2; ++x) {
           wait_for(__shfl_sync(~0u, holder, stage));
           const bool last_values = x == 1 && s == 0 && tail;
-          const uint32_t bar = ptx::smem_u32(last_values ? tail_bar : full_bar + stage);
+          const uint32_t bar = ptx::smem_u32((last_values ? tail_bar : full_bar) + stage);
           if (lane == 0 && alive) ptx::mbar_arrive_expect_tx(bar, held * p.box_rows * D * 2);
           __syncwarp();
           if (lane < held && alive)
             for (int h = 0; h < kHalves; ++h)
               ptx::tma_load_4d(ring_base + stage * kTileBytes + h * kHalfBytes + lane * p.box_rows * 128,
                                x == 0 ? &tmap_k : &tmap_v, bar, h * 64, it.kv, at, mine);
-          if (last_values) ++tails;
+          if (last_values) {
+            tail_phase ^= (tails >> stage & 1u) << stage;      // of the last copy
+            tails |= 1u << stage;
+          }
           // signals of an item: the first scores; then each step's values together with the next one's scores
           if (lane == stage) holder = signal + s + x;
           if (++stage == kStages) {
@@ -441,7 +444,8 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     __syncwarp();
     if (lane == 0) {
       if (*abort_flag != 0) ptx::drain_ring(full_bar, kStages, stage, phase);
-      if (*abort_flag != 0 && tails > 0) ptx::drain_ring(tail_bar, 1, 1, (tails - 1) & 1);
+      for (int s = 0; s < kStages; ++s)
+        if (*abort_flag != 0 && (tails >> s & 1u) != 0u) ptx::drain_ring(tail_bar + s, 1, 1, tail_phase >> s & 1u);
       if (*abort_flag != 0 && queries > 0) ptx::drain_ring(q_bar, 1, 1, (queries - 1) & 1);
     }
   } else if (warp == 8) {
@@ -530,14 +534,15 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     // Behind the last key the last V tile holds another sequence's rows or whatever the page did, and 0 * NaN is NaN: cleared
     // up to the next multiple of 16, which is what the products read.
     int stage = 0;
-    uint32_t tails = 0;
+    uint32_t tail_phase = 0;      // a bit for each place of the ring: the next copy's
     Item it;
     while (fetch(it)) {
       const int steps = it.hi - it.lo;
       if (steps > 0 && it.hi * kRows > it.m) {
-        if (alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(tail_bar), tails & 1, abort_flag));
-        ++tails;
         const int place = stage + 1 == kStages ? 0 : stage + 1, from = it.m - (it.hi - 1) * kRows;
+        // A barrier for each place: the next item's last values may be on their way before these are there.
+        if (alive) alive = ptx::warp_all(ptx::mbar_wait(ptx::smem_u32(tail_bar + place), tail_phase >> place & 1u, abort_flag));
+        tail_phase ^= 1u << place;
         for (int e = lane; e < (((from + 15) & ~15) - from) * (D / 8); e += 32) {
           const int r = from + e / (D / 8), c = e % (D / 8);
           *reinterpret_cast<uint4*>(ring + place * kTileBytes + (c >> 3) * kHalfBytes + r * 128 + (c & 7) * 16) =
