@@ -441,6 +441,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       q_free = signal + steps - 1;
       signal += steps + 1;
     }
+    wait_for(signal - 1);      // no signal is on its way to a barrier of a CTA that has ended
     __syncwarp();
     if (lane == 0) {
       if (*abort_flag != 0) ptx::drain_ring(full_bar, kStages, stage, phase);
