@@ -64,10 +64,9 @@ constexpr int kItems = 4;                         // places for items that are o
 constexpr int kSignals = 8;                       // more than the products can be ahead of the copies: stages / 2 + 1
 
 template <int D>
-constexpr int stages() { return D == 128 ? 4 : 8; }
-constexpr int kStageOut = 32 * 128;               // a warp's output on its way: 32 rows x 128 bytes
+constexpr int stages() { return D == 128 ? 5 : 10; }
 template <int D>
-constexpr int smem_bytes() { return (2 + stages<D>()) * kRows * D * 2 + 8 * kStageOut + kCtrlBytes; }
+constexpr int smem_bytes() { return (2 + stages<D>()) * kRows * D * 2 + kCtrlBytes; }
 
 // The queries of one sequence that a CTA works on, and the part of the sequence's keys.
 struct alignas(16) Item {
@@ -232,8 +231,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
   constexpr int kStages = stages<D>();
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* ring = smem + 2 * kTileBytes;
-  uint8_t* out_stage = ring + kStages * kTileBytes;
-  uint8_t* ctrl = out_stage + 8 * kStageOut;
+  uint8_t* ctrl = ring + kStages * kTileBytes;
   Item* items = reinterpret_cast<Item*>(ctrl);              // [items]
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(items + kItems);   // [stages] a K or V tile is there
   uint64_t* free_bar = full_bar + kStages;                  // [signals], in turn: products up to a step are done
@@ -562,63 +560,55 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     const int row_query = row * p.group_inverse >> 16;      // row / group
     const uint32_t lanes = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t col_s = lanes + t * kRows, col_o = lanes + kColO + t * kRows;
-    uint8_t* const my_stage = out_stage + warp * kStageOut;
     const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
     uint32_t s_phase = 0, o_phase = 0;
-    // 128 bytes of each row at a time go through shared memory: eight lanes write a line of a row together
-    const auto staged = [&](int i) { return reinterpret_cast<uint4*>(my_stage + lane * 128 + ((i ^ (lane & 7)) << 4)); };
-    const auto store = [&](uint8_t* base, int rows, int row_bytes, int query_bytes, int from, int bytes) {
-      __syncwarp();
+    // A thread has its row's values one after another: it writes whole sectors of 32 bytes, where rows begin on such boundaries.  (By way
+    // of shared memory, in whole lines, it took as long, and a place of the ring.)
+    const auto write = [&](uint8_t* row, const uint32_t* v, int from, int bytes) {      // values `from` to from + 32 of a row
+      if (((reinterpret_cast<uintptr_t>(row) | bytes) & 31u) == 0u) {
+        if (from < bytes) ptx::st_global_32(row + from, v);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = 4 * i + (lane >> 3), all = (warp & 3) * 32 + r, at = from + (lane & 7) * 16;
-        const uint4 v = *reinterpret_cast<const uint4*>(my_stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-        if (all < rows && at < bytes)
-          *reinterpret_cast<uint4*>(base + all * row_bytes + (all * p.group_inverse >> 16) * query_bytes + at) = v;
+        for (int i = 0; i < 2; ++i)
+          if (from + 16 * i < bytes) *reinterpret_cast<uint4*>(row + from + 16 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
       }
-      __syncwarp();
     };
     // An item's result, where tile t has one; `any`: there are sums.
     const auto output = [&](const Item& it, bool any, bool sees, float top, float sum) {
-      const int to = it.first + t * p.tile_tokens, rows = min(it.n - to, p.tile_tokens) * p.group;      // real ones
+      const int to = it.first + t * p.tile_tokens;
+      const bool real = row < min(it.n - to, p.tile_tokens) * p.group;
       if (it.pieces > 1) {
-        const int64_t at = (static_cast<int64_t>(it.slot) * p.kv_heads + it.kv) * 2 * kRows + t * kRows;
-        if (row < rows) p.part_ml[at + row] = make_float2(top, sum);
-#pragma unroll
+        const int64_t at = (static_cast<int64_t>(it.slot) * p.kv_heads + it.kv) * 2 * kRows + t * kRows + row;
+        if (real) p.part_ml[at] = make_float2(top, sum);
+#pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           if (!any) break;
           uint32_t o[32];
           ptx::tmem_ld_32x32b_x32(col_o + 32 * c, o);
           ptx::tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 8; ++i) *staged(i) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-          store(reinterpret_cast<uint8_t*>(p.part_o + at * D), rows, D * 4, 0, c * 128, D * 4);
+          for (int i = 0; i < 4; ++i)
+            if (real) write(reinterpret_cast<uint8_t*>(p.part_o + at * D), o + 8 * i, c * 128 + 32 * i, D * 4);
         }
         return;
       }
       // rows of one query are neighbours; the next query is all heads further
-      uint8_t* base = reinterpret_cast<uint8_t*>(static_cast<T*>(p.out) +
-                                                 (static_cast<int64_t>(it.row0 + to) * p.heads + it.kv * p.group) * p.dim);
+      uint8_t* to_row = reinterpret_cast<uint8_t*>(
+          static_cast<T*>(p.out) + (static_cast<int64_t>(it.row0 + to + row_query) * p.heads + it.kv * p.group + row - row_query * p.group) * p.dim);
       const float inv = inverse(sum);
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t o[32];
-          if (any) {
-            ptx::tmem_ld_32x32b_x32(col_o + 64 * c + 32 * h, o);
-            ptx::tmem_ld_wait();
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t v[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              v[j] = sees ? pack16<T>(__uint_as_float(o[8 * i + 2 * j]) * inv, __uint_as_float(o[8 * i + 2 * j + 1]) * inv) : 0u;
-            *staged(4 * h + i) = make_uint4(v[0], v[1], v[2], v[3]);
-          }
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32], v[16];
+        if (any) {
+          ptx::tmem_ld_32x32b_x32(col_o + 32 * c, o);
+          ptx::tmem_ld_wait();
         }
-        store(base, rows, p.dim * 2, (p.heads - p.group) * p.dim * 2, c * 128, p.dim * 2);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          v[i] = sees ? pack16<T>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv) : 0u;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (real) write(to_row, v + 8 * i, c * 64 + 32 * i, p.dim * 2);
       }
     };
     uint32_t x[kRows], e16[kRows / 2];
