@@ -733,6 +733,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
           ptx::tc_fence_after_sync();
         }
         output(items[done], done_any, done_sees, done_top, done_sum);
+        __syncwarp();      // all lanes have read the item: its place is free
         if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(read_bar + done));
       }
       if (end) break;
