@@ -852,7 +852,9 @@ __global__ void __launch_bounds__(kJoinThreads) attn_prefill_join_kernel(const P
         for (int i = 0; i < 8; ++i) {
           const int c = min(c1 + i, 31);
           const float f = __shfl_sync(~0u, weight, c), m = __shfl_sync(~0u, ml.x, c), s = __shfl_sync(~0u, ml.y, c);
-          if (c1 + i >= count || m == -INFINITY) continue;      // a piece of which the row sees nothing: its sums may be anything
+          // A piece of which the row sees nothing: its sums may be anything.  (NaN scores beside hidden ones leave a maximum of -inf as well,
+          // and a sum of NaN, which is the row's.)
+          if (c1 + i >= count || (m == -INFINITY && s == 0.f)) continue;
           l += f * s;
           acc.x += v[i].x * f, acc.y += v[i].y * f, acc.z += v[i].z * f, acc.w += v[i].w * f;
         }
