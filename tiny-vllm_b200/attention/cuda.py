@@ -228,7 +228,7 @@ def copy_pages(kv_cache: torch.Tensor, src: list[int], dst: list[int]) -> None:
     """
     what = "copy_pages"
     if not isinstance(src, (list, tuple)) or not isinstance(dst, (list, tuple)) \
-            or not all(isinstance(i, int) for i in (*src, *dst)):
+            or not all(isinstance(i, int) and not isinstance(i, bool) for i in (*src, *dst)):
         raise ValueError(f"{what} expects lists of page numbers on the host")
     if len(src) != len(dst):
         raise ValueError(f"{what}: {len(src)} sources and {len(dst)} destinations")
