@@ -484,7 +484,8 @@ typedef struct {
 typedef struct {
   b200q_view q;          /* [tokens][heads][dim]; the page stride is not used                        */
   b200q_view k, v;       /* packed: [key_tokens][kv_heads][dim]; paged: [pages][page_size][kv_heads][dim] */
-  void* out;             /* dense [tokens][heads][dim]; rows behind the last sequence are left alone  */
+  void* out;             /* dense [tokens][heads][dim], no memory of q, k or v (decode: q itself is allowed);
+                            rows behind the last sequence are left alone                              */
   const int32_t* cu_q;   /* prefill: [sequences + 1], where each sequence's queries begin             */
   const int32_t* cu_k;   /* prefill: [sequences + 1], the same of its keys (paged: only the differences count) */
   const int32_t* lengths;/* decode: [sequences], keys of each sequence, its new token among them       */

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from attn_util import Paged, check, cumulated, packed_reference, rows
+from gpu_util import device_status_ok
 from tiny_vllm_b200.attention import decode_attention, prefill_attention
 
 pytestmark = pytest.mark.gpu
@@ -48,3 +49,67 @@ def test_maxima_that_move_by_far_more_than_a_weights_range(dtype, dim, n, m, sha
     check(prefill_attention(q, paged.k, paged.v, cumulated([n]), cumulated([m]), n, m, scale=1.0, block_tables=paged.tables), want, tol)
     lengths = torch.tensor([m], dtype=torch.int32, device="cuda")
     check(decode_attention(q[-1:], paged.k, paged.v, lengths, paged.tables, scale=1.0), want[-1:], tol[-1:])
+
+
+@pytest.mark.parametrize("n,m", [(300, 300), (3, 6000)], ids=["whole", "cut"])
+@pytest.mark.parametrize("dtype,power", [(BF, 24), (BF, 31), (BF, 60), (BF, 120), (HF, 22), (HF, 24), (HF, 28)])
+def test_scores_of_any_size(dtype, power, n, m):
+    # Scores are whole multiples of 2^power, zero among them, of either sign and exact: a row is the mean of the values of its
+    # largest ones, all other weights being 2^-(2^22) or less.  Courses rise, fall, do both, and rise in a tile's last columns.
+    dim, heads, kv = 64, 4, 2
+    gen = generator(power)
+    j = torch.arange(m, device="cuda")
+    q, unit = torch.zeros(n, heads, dim, device="cuda"), torch.zeros(dim, device="cuda")
+    if dtype == BF:
+        q[:, :, 5], unit[5] = 2.0 ** (power - power // 2), 2.0 ** (power // 2)
+    else:      # as many components as it takes: 2^14 2^8 each
+        q[:, :, :2 ** (power - 22)], unit[:2 ** (power - 22)] = 2.0 ** 14, 2.0 ** 8
+    lengths = torch.tensor([m], dtype=torch.int32, device="cuda")
+    for course in (j // 50 - 3, -(j // 50), torch.full_like(j, -1), torch.full_like(j, 77), (j * 7) % 53 - 60,
+                   20 - (j - m // 2).abs() // 40, (j % 128 >= 100).int() - 3, j % 97 - j // 31):
+        course = course.clamp(-127, 127)
+        k = course[:, None, None] * unit.expand(m, kv, dim)
+        v = rows(gen, m, kv, dim, dtype)
+        seen = torch.ones(n, m, dtype=torch.bool, device="cuda").tril(m - n)
+        top = torch.where(seen, course, -1000).amax(1, keepdim=True)
+        p = (seen & (course == top)).double()
+        p = p / p.sum(1, keepdim=True)
+        want = torch.einsum("nm,mhd->nhd", p, v.double()).repeat_interleave(2, 1)
+        a = torch.einsum("nm,mhd->nhd", p, v.double().abs()).repeat_interleave(2, 1)
+        # weights are 1, up to the exponential's 2^-16 and a factor that a row's sums share; then sums over m keys in 32 bits, the rounding
+        tol = torch.finfo(dtype).eps / 2 * want.abs() + (2.0 ** -15 + m * 2.0 ** -23) * 1.01 * a + 2.0 ** -25
+        kk = k.to(dtype)
+        assert torch.equal(kk.float(), k)
+        check(prefill_attention(q.to(dtype), kk, v, cumulated([n]), cumulated([m]), n, m, scale=1.0), want, tol)
+        paged = Paged(gen, kk, v, [m], 64)
+        check(prefill_attention(q.to(dtype), paged.k, paged.v, cumulated([n]), cumulated([m]), n, m, scale=1.0,
+                                block_tables=paged.tables), want, tol)
+        check(decode_attention(q[-1:].to(dtype), paged.k, paged.v, lengths, paged.tables, scale=1.0), want[-1:], tol[-1:])
+    assert device_status_ok()
+
+
+def test_queries_that_are_overwritten_by_their_results():
+    # scores far from zero and near it: rows of the first kind are worked on twice
+    queries, keys = [300, 70], [300, 4000]
+    gen = generator(3)
+    q, k, v = rows(gen, 370, 8, 64, BF, 2.0), rows(gen, 4300, 2, 64, BF), rows(gen, 4300, 2, 64, BF)
+    q[100:200, :, 3] = 2.0 ** 20
+    q[340:350, 3, 3] = -2.0 ** 20
+    want = prefill_attention(q, k, v, cumulated(queries), cumulated(keys), 300, 4000)
+    assert not torch.equal(want[100:200], want[:100])
+    out = q.clone()
+    got = prefill_attention(out, k, v, cumulated(queries), cumulated(keys), 300, 4000, out=out)
+    assert got.data_ptr() == out.data_ptr() and torch.equal(got, want)
+    parts = torch.cat([q, q], 1)      # strided queries over which a dense result is laid
+    over = parts.view(-1)[:q.numel()].view_as(q)
+    got = prefill_attention(parts[:, 8:], k, v, cumulated(queries), cumulated(keys), 300, 4000, out=over)
+    assert torch.equal(got, want)
+    last = torch.tensor(keys, dtype=torch.int32, device="cuda")
+    paged = Paged(gen, k, v, keys, 16)
+    one = q[[299, 369]].clone()
+    want = decode_attention(one, paged.k, paged.v, last, paged.tables)
+    parts = torch.cat([one, one], 1)
+    got = decode_attention(one, paged.k, paged.v, last, paged.tables, out=one)
+    assert torch.equal(got, want)
+    got = decode_attention(parts[:, 8:], paged.k, paged.v, last, paged.tables, out=parts.view(-1)[:one.numel()].view_as(one))
+    assert torch.equal(got, want)

@@ -14,8 +14,8 @@ over ``j <= i + m - n`` (``causal``) or all ``j < m``; zeros where that leaves n
 are fp32; the softmax weights are rounded to the tensors' type for the second product, as is the result.  What
 keys hold that a row does not see does not matter, NaN and infinities included, with one exception: a non-finite
 *value* at a later position of the same sequence may reach rows up to 142 positions before it, as zero times
-infinity does in any matrix product.  Scores ``scale * q . k`` are fp32 and may reach 2^24 in magnitude, from where on
-fp32 does not tell neighbours apart; rows of prompts with larger ones may be wrong.
+infinity does in any matrix product.  Scores ``scale * q . k`` are fp32 and may be of any size up to 2^127; prompts take
+some hundred times as long over rows with scores beyond 700,000, which no trained model has.
 
 ``float16`` or ``bfloat16``; ``dim`` a multiple of 8 up to 128; up to 128 query heads per key head; pages of a
 multiple of 16 positions.  Heads, tokens and pages may stand apart (strides of a multiple of 8 elements).  Calls run on
@@ -92,6 +92,12 @@ def _check_out(what: str, q: torch.Tensor, out: torch.Tensor | None) -> None:
         raise RuntimeError(f"{what}: out must be a contiguous {list(q.shape)} {q.dtype} tensor on {q.device}")
 
 
+def _share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    def end(t: torch.Tensor) -> int:
+        return t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+    return a.data_ptr() < end(b) and b.data_ptr() < end(a)
+
+
 def _finish(what: str, out, *tensors):
     if out is None:
         _require_one_gpu(what, *tensors)
@@ -148,7 +154,10 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seql
         k, v = _aligned(k), _aligned(v)
     else:
         block_tables = block_tables.contiguous()
-    o = _native().attention(_aligned(q), k, v, cu_seqlens_q.contiguous(), cu_seqlens_k.contiguous(), None, block_tables,
+    q = _aligned(q)
+    if out is not None and _share_memory(q, out):
+        q = q.clone(memory_format=torch.contiguous_format)      # the kernel may read queries again behind their results
+    o = _native().attention(q, k, v, cu_seqlens_q.contiguous(), cu_seqlens_k.contiguous(), None, block_tables,
                             max_seqlen_q, max_seqlen_k, scale, causal, out)
     return _finish(what, o, q, k, v, cu_seqlens_q, cu_seqlens_k, block_tables)
 
@@ -184,7 +193,10 @@ def decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     _check_out(what, q, out)
     if q.numel() == 0:
         return torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
-    o = _native().attention(_aligned(q), k_cache, v_cache, None, None, context_lens.contiguous(),
+    q = _aligned(q)
+    if out is not None and _share_memory(q, out) and not (q.data_ptr() == out.data_ptr() and q.is_contiguous()):
+        q = q.clone(memory_format=torch.contiguous_format)
+    o = _native().attention(q, k_cache, v_cache, None, None, context_lens.contiguous(),
                             block_tables.contiguous(), 1, 0, scale, True, out)
     return _finish(what, o, q, k_cache, v_cache, context_lens, block_tables)
 

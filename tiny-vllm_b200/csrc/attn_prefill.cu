@@ -56,6 +56,7 @@ constexpr int kCtrlBytes = 1024;
 constexpr int kTmemCols = 512;
 constexpr uint32_t kColO = 256;
 constexpr float kMost = 4096.f, kMostLog2 = 12.f;  // the largest weight
+constexpr float kFar = 1048576.f;                 // rows with larger maxima go to row_by_row
 constexpr int kMinChunk = 8;                      // tiles of keys: the shortest piece that an item is cut into
 constexpr int kFirstGroups = 6;                   // of 16 keys, whose weights are announced first
 constexpr int kChecked = 48;                      // pairs of weights whose sum says whether the maximum follows
@@ -86,6 +87,7 @@ struct Header {
 };
 
 struct PrefillParams {
+  b200q_view q, k, v;   // for row_by_row
   void* out;
   const int32_t *cu_q, *cu_k, *tables;
   int64_t table_stride;
@@ -221,10 +223,135 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
   if (threadIdx.x == 0) p.header->joins = joins;
 }
 
+// Where key `pos` of an item stands in x; -1: in a page outside of the cache, which counts as zeros, or behind the last key.
+__device__ __forceinline__ int64_t place_of(const PrefillParams& p, const Item& it, const b200q_view& x, int pos) {
+  if (pos >= it.m) return -1;
+  if (p.page_size == 0) return static_cast<int64_t>(it.key0 + pos) * x.token + it.kv * x.head;
+  const int page = p.tables[it.b * p.table_stride + pos / p.page_size];
+  return page < 0 || page >= p.pages ? -1 : page * x.page + pos % p.page_size * x.token + it.kv * x.head;
+}
+
+// A warp's 32 rows of tile t of an item (or of a piece of it) once more, the result written over the former one, where a maximum is far from zero.
+// Exponents are scale (x - max x), and weights stay in fp32.  Scores by mma.sync, 16 rows x 8 keys at a time, straight from memory.  Rare, so it
+// may be slow: 8192 tokens of 32 / 8 heads of 128 whose scores are all far take 49 ms, 2700 cycles a key of an item.  A function of its
+// own, since its code between the other steps costs these up to 9 %.
+template <typename T, int D>
+__device__ __noinline__ void row_by_row(const PrefillParams& p, const Item& it, int t, int my_row) {
+  const int lane = threadIdx.x & 31, gid = lane >> 2, tid = lane & 3, row0 = my_row - lane;
+  const auto limit_of = [&](int row) {      // keys of the piece that a row sees; -1: no row
+    const int of = row / p.group, query = it.first + t * p.tile_tokens + of;
+    return of < p.tile_tokens && query < it.n ? min(seen_by(p, it, query), it.hi * kRows) : -1;
+  };
+  __syncwarp();      // the former result was written by other lanes
+#pragma unroll 1
+  for (int block = 0; block < 32; block += 16) {
+    int row[2], limit[2];
+    float most[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, o[D / 8][4];
+    const T* q[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      row[h] = row0 + block + gid + 8 * h, limit[h] = limit_of(row[h]);
+      const int query = it.row0 + it.first + t * p.tile_tokens + row[h] / p.group, head = it.kv * p.group + row[h] % p.group;
+      q[h] = static_cast<const T*>(p.q.data) + (limit[h] < 0 ? 0 : query * p.q.token + head * p.q.head);
+    }
+    uint32_t a[D / 16][4];
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = 16 * k + 8 * (i >> 1) + 2 * tid;
+        a[k][i] = limit[i & 1] >= 0 && d < p.dim ? *reinterpret_cast<const uint32_t*>(q[i & 1] + d) : 0u;
+      }
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+    const int all = __reduce_max_sync(~0u, max(limit[0], limit[1]));
+#pragma unroll 1
+    for (int j = it.lo * kRows; j < all; j += 8) {
+      const int64_t k_at = place_of(p, it, p.k, j + gid), v_at = place_of(p, it, p.v, j + gid);      // of the key that a lane has in a product
+      const T* key = static_cast<const T*>(p.k.data) + (k_at < 0 ? 0 : k_at);
+      float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        uint32_t b[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int d = 16 * k + 8 * i + 2 * tid;
+          b[i] = k_at >= 0 && d < p.dim ? *reinterpret_cast<const uint32_t*>(key + d) : 0u;
+        }
+        mma_16<T>(s, a[k][0], a[k][1], a[k][2], a[k][3], b[0], b[1]);
+      }
+      float f[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {      // keys 2 tid and 2 tid + 1 of rows gid, gid + 8
+        float to = most[h];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (j + 2 * tid + i >= limit[h]) s[2 * h + i] = -INFINITY;
+          to = fmaxf(to, s[2 * h + i]);
+        }
+        to = fmaxf(to, __shfl_xor_sync(~0u, to, 1));
+        to = fmaxf(to, __shfl_xor_sync(~0u, to, 2));
+        f[h] = to == most[h] ? 1.f : exp2_approx((most[h] - to) * p.scale_log2);
+        most[h] = to;
+        const float base = to == -INFINITY ? 0.f : to;
+        sum[h] *= f[h];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          s[2 * h + i] = exp2_approx((s[2 * h + i] - base) * p.scale_log2);
+          sum[h] += s[2 * h + i];
+        }
+      }
+      if (__any_sync(~0u, f[0] != 1.f || f[1] != 1.f)) {
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) o[n][0] *= f[0], o[n][1] *= f[0], o[n][2] *= f[1], o[n][3] *= f[1];
+      }
+#pragma unroll 1
+      for (int i = 0; i < 8; ++i) {
+        const int from = (lane & 28) | (i >> 1);
+        const float w0 = __shfl_sync(~0u, i & 1 ? s[1] : s[0], from), w1 = __shfl_sync(~0u, i & 1 ? s[3] : s[2], from);
+        const int64_t at = __shfl_sync(~0u, v_at, 4 * i);
+        const T* value = static_cast<const T*>(p.v.data) + at + 2 * tid;
+        if (at < 0) continue;
+        const bool sees0 = j + i < limit[0], sees1 = j + i < limit[1];
+        uint32_t v[D / 8];
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) v[n] = 8 * n + 2 * tid < p.dim ? *reinterpret_cast<const uint32_t*>(value + 8 * n) : 0u;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) {
+          const float x = static_cast<float>(reinterpret_cast<const T*>(&v[n])[0]), y = static_cast<float>(reinterpret_cast<const T*>(&v[n])[1]);
+          if (sees0) o[n][0] = fmaf(w0, x, o[n][0]), o[n][1] = fmaf(w0, y, o[n][1]);
+          if (sees1) o[n][2] = fmaf(w1, x, o[n][2]), o[n][3] = fmaf(w1, y, o[n][3]);
+        }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      sum[h] += __shfl_xor_sync(~0u, sum[h], 1);
+      sum[h] += __shfl_xor_sync(~0u, sum[h], 2);
+      if (limit[h] < 0) continue;
+      if (it.pieces > 1) {
+        const int64_t at = (static_cast<int64_t>(it.slot) * p.kv_heads + it.kv) * 2 * kRows + t * kRows + row[h];
+        if (tid == 0) p.part_ml[at] = make_float2(most[h] * p.scale_log2, sum[h]);
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+          *reinterpret_cast<float2*>(p.part_o + at * D + 8 * n + 2 * tid) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+      } else {
+        const float inv = inverse(sum[h]);
+        const int query = it.row0 + it.first + t * p.tile_tokens + row[h] / p.group, head = it.kv * p.group + row[h] % p.group;
+        T* to = static_cast<T*>(p.out) + (static_cast<int64_t>(query) * p.heads + head) * p.dim + 2 * tid;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+          if (8 * n < p.dim) *reinterpret_cast<uint32_t*>(to + 8 * n) = pack16<T>(o[n][2 * h] * inv, o[n][2 * h + 1] * inv);
+      }
+    }
+    __syncwarp();
+  }
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
-                    const __grid_constant__ CUtensorMap tmap_v, const PrefillParams p) {
+                    const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ PrefillParams p) {
   constexpr int kHalves = D / 64;
   constexpr int kHalfBytes = kRows * 128;
   constexpr int kTileBytes = kRows * D * 2;
@@ -614,6 +741,10 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     uint32_t x[kRows], e16[kRows / 2];
     uint64_t part[2];
     float top = 0.f, most[4];
+    // An exponent is scale x - top, with top = scale max x rounded: an error of a factor that a row's weights share, 2^(2^-4) where top is
+    // kFar, but without bounds beyond.  Such a row is marked by an infinite maximum, its weights come out as 0, and row_by_row
+    // takes it once more behind the output.
+    const auto marked = [&](float x) { return fabsf(x) > kFar && x != -INFINITY ? INFINITY : x; };
     // Weights of pairs [from, to), eight at a time; sums, conversions and maxima (of the scores behind kChecked) of eight
     // stand beside the exponentials of the next.  The exponential unit gives 16 results a cycle for the SM; every eighth pair
     // goes through the multipliers instead (8 x 1024 tokens: every 4th 96 us, every 8th 93).
@@ -713,7 +844,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
           for (int i = 0; i < 4; ++i) most[i] = max3(most[i], __uint_as_float(x[c + 2 * i]), __uint_as_float(x[c + 2 * i + 1]));
 #pragma unroll
         for (int i = 0; i < 4; ++i) most[i] = fmaxf(most[i], __uint_as_float(x[kRows - 4 + i]));
-        top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * p.scale_log2;
+        top = marked(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * p.scale_log2);
         part[0] = part[1] = pair(0.f, 0.f);
         weights(0, 32);
         ptx::tmem_st_32x32b_x32(col_s, *reinterpret_cast<uint32_t(*)[32]>(e16));
@@ -733,6 +864,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
           ptx::tc_fence_after_sync();
         }
         output(items[done], done_any, done_sees, done_top, done_sum);
+        if (__any_sync(~0u, done_any && done_top == INFINITY)) row_by_row<T, D>(p, items[done], t, row);
         __syncwarp();      // all lanes have read the item: its place is free
         if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(read_bar + done));
       }
@@ -792,7 +924,7 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
 #pragma unroll
           for (int i = 0; i < 2 * kChecked; i += 2) most[i & 2] = max3(most[i & 2], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
           const float to = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * p.scale_log2;
-          raise(limit > begin ? fmaxf(to, top) : top);
+          raise(marked(limit > begin ? fmaxf(to, top) : top));
           part[0] = part[1] = pair(0.f, 0.f);
           weights(0, kChecked);
         }
@@ -940,6 +1072,7 @@ int launch_attn_prefill(const b200q_attention& a, void* workspace, int* status, 
   const Plan plan = make_plan(a);
   if (plan.units * a.kv_heads > INT_MAX / 2) return B200Q_ERR_BAD_SHAPE;
   PrefillParams p{};
+  p.q = a.q, p.k = a.k, p.v = a.v;
   p.out = a.out;
   p.cu_q = a.cu_q, p.cu_k = a.cu_k, p.tables = a.tables, p.table_stride = a.table_stride;
   p.tokens = a.tokens, p.key_tokens = a.key_tokens, p.sequences = a.sequences;

@@ -429,6 +429,15 @@ bool view_of(const at::Tensor& t, b200q_view* out) {
   out->page = n > 3 && t.size(n - 4) > 1 ? t.stride(n - 4) : 0;
   return out->head % 8 == 0 && out->token % 8 == 0 && out->page % 8 == 0;
 }
+// whether the memory from their first to their last elements overlaps (strides are not negative)
+bool share_memory(const at::Tensor& a, const at::Tensor& b) {
+  const auto end = [](const at::Tensor& t) {
+    int64_t last = 1;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    return static_cast<const char*>(t.data_ptr()) + last * t.element_size();
+  };
+  return a.data_ptr() < end(b) && b.data_ptr() < end(a);
+}
 // an int32 tensor on `device`, dense in its last dimension
 inline bool ints(const at::Tensor* t, int64_t dim, const at::Device& device) {
   return t != nullptr && t->scalar_type() == at::kInt && t->device() == device && t->dim() == dim &&
@@ -506,6 +515,8 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   } else {
     const at::Tensor* given = tensor_of(args[11]);
     if (!dense(given, type, device) || given->sizes() != q->sizes()) Py_RETURN_NONE;
+    // (a decode step's queries may be overwritten row by row)
+    if (share_memory(*q, *given) && !(decode && q->data_ptr() == given->data_ptr() && q->is_contiguous())) Py_RETURN_NONE;
     out = *given;
   }
   a.out = out.data_ptr();
