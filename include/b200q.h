@@ -466,9 +466,8 @@ int b200q_w8a8_gemm_noalloc(const int8_t* xq, const float* a_scales, const int8_
  *
  * over the keys j that row i sees.  In a sequence with n queries and m keys (0 <= n, m; the queries
  * are the last n of m positions) causal attention shows row i the keys j <= i + m - n; without
- * `causal` every row sees all m.  A row that sees no key, or only scores of -infinity, gives zeros.  Keys that a row does not see do not
- * reach it whatever they hold, with one exception: a non-finite value v of a later position of the same sequence
- * may make the rows up to 142 positions before it non-finite, as zero times infinity does in any matrix product.
+ * `causal` every row sees all m.  A row that sees no key, or only scores of -infinity, gives zeros.  Keys
+ * and values that a row does not see do not reach it, whatever they hold.
  * Sums and softmax statistics are fp32; the weights exp(s - top) are rounded to T once, as operands of the
  * second product, and the result once.
  *

@@ -12,10 +12,9 @@ With ``G = heads / kv_heads`` and a sequence of ``n`` queries and ``m`` keys, th
 
 over ``j <= i + m - n`` (``causal``) or all ``j < m``; zeros where that leaves no key, or only scores of -infinity.  Sums and softmax statistics
 are fp32; the softmax weights are rounded to the tensors' type for the second product, as is the result.  What
-keys hold that a row does not see does not matter, NaN and infinities included, with one exception: a non-finite
-*value* at a later position of the same sequence may reach rows up to 142 positions before it, as zero times
-infinity does in any matrix product.  Scores ``scale * q . k`` are fp32 and may be of any size up to 2^127; prompts take
-some hundred times as long over rows with scores beyond 700,000, which no trained model has.
+keys and values hold that a row does not see does not matter, NaN and infinities included.  Scores ``scale * q . k`` are
+fp32 and may be of any size up to 2^127.  Two things that no healthy model has make prompts slow, a hundred times for the rows
+concerned: scores beyond 700,000, and values that are not finite up to 255 positions behind a row that does not see them.
 
 ``float16`` or ``bfloat16``; ``dim`` a multiple of 8 up to 128; up to 128 query heads per key head; pages of a
 multiple of 16 positions.  Heads, tokens and pages may stand apart (strides of a multiple of 8 elements).  Calls run on

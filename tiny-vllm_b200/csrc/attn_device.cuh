@@ -41,6 +41,15 @@ __device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// Eight 16-bit values on a 16-byte boundary, as fp32.
+template <typename T>
+__device__ __forceinline__ void unpack8(const T* p, float (&x)[8]) {
+  const uint4 v = *reinterpret_cast<const uint4*>(p);
+  const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(e[i]);
+}
+
 // 2^x to two units in the last place, 0 for -inf; results below the smallest normal number are flushed to zero.
 __device__ __forceinline__ float exp2_approx(float x) {
   float r;

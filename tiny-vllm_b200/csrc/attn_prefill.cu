@@ -231,17 +231,36 @@ __device__ __forceinline__ int64_t place_of(const PrefillParams& p, const Item& 
   return page < 0 || page >= p.pages ? -1 : page * x.page + pos % p.page_size * x.token + it.kv * x.head;
 }
 
-// A warp's 32 rows of tile t of an item (or of a piece of it) once more, the result written over the former one, where a maximum is far from zero.
-// Exponents are scale (x - max x), and weights stay in fp32.  Scores by mma.sync, 16 rows x 8 keys at a time, straight from memory.  Rare, so it
-// may be slow: 8192 tokens of 32 / 8 heads of 128 whose scores are all far take 49 ms, 2700 cycles a key of an item.  A function of its
-// own, since its code between the other steps costs these up to 9 %.
+// A warp's 32 rows of tile t of an item (or of a piece of it) once more, the result written over the former one: where a maximum is
+// far from zero (odd = 2), or where sums are not finite though the weights are (1) and a value that is not finite stands behind what a
+// row sees (its weight is 0, and 0 * inf is NaN).  Exponents are scale (x - max x), weights stay in fp32, and only what a row sees
+// is multiplied.  Scores by mma.sync, 16 rows x 8 keys at a time, straight from memory.  Rare, so it may be slow: 8192 tokens of
+// 32 / 8 heads of 128 whose scores are all far take 49 ms, 2700 cycles for each of an item's keys (beyond 700,000 of them the
+// other warps' waits run out, and the call ends with a device status).  A function of its own: the same work between the other
+// steps cost these up to 9 %.
 template <typename T, int D>
-__device__ __noinline__ void row_by_row(const PrefillParams& p, const Item& it, int t, int my_row) {
+__device__ __noinline__ void row_by_row(const PrefillParams& p, const Item& it, int t, int my_row, int odd) {
   const int lane = threadIdx.x & 31, gid = lane >> 2, tid = lane & 3, row0 = my_row - lane;
   const auto limit_of = [&](int row) {      // keys of the piece that a row sees; -1: no row
     const int of = row / p.group, query = it.first + t * p.tile_tokens + of;
     return of < p.tile_tokens && query < it.n ? min(seen_by(p, it, query), it.hi * kRows) : -1;
   };
+  if (!__any_sync(~0u, odd == 2)) {
+    // is there a value at all that is not finite, behind the fewest keys that a row sees?
+    const int mine = limit_of(row0 + lane), pieces = p.dim / 8, fewest = __reduce_min_sync(~0u, mine < 0 ? INT_MAX : mine);
+    const int from = max(fewest, it.lo * kRows), keys = min(it.m, (it.hi - it.part[t].skip) * kRows) - from;
+    float zero = 0.f;
+#pragma unroll 1
+    for (int e0 = 0; e0 < keys * pieces; e0 += 32) {
+      const int e = min(e0 + lane, keys * pieces - 1);
+      const int64_t at = place_of(p, it, p.v, from + e / pieces);
+      float x[8];
+      unpack8<T>(static_cast<const T*>(p.v.data) + (at < 0 ? 0 : at) + e % pieces * 8, x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) zero = at < 0 ? zero : fmaf(x[i], 0.f, zero);
+    }
+    if (!__any_sync(~0u, zero != 0.f)) return;      // (NaN, too, is not 0)
+  }
   __syncwarp();      // the former result was written by other lanes
 #pragma unroll 1
   for (int block = 0; block < 32; block += 16) {
@@ -700,10 +719,15 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
           if (from + 16 * i < bytes) *reinterpret_cast<uint4*>(row + from + 16 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
       }
     };
-    // An item's result, where tile t has one; `any`: there are sums.
+    // An item's result, where tile t has one; `any`: there are sums.  Returns what row_by_row has to know of the row: 0 where it is done.
     const auto output = [&](const Item& it, bool any, bool sees, float top, float sum) {
       const int to = it.first + t * p.tile_tokens;
       const bool real = row < min(it.n - to, p.tile_tokens) * p.group;
+      uint64_t zero[4] = {0, 0, 0, 0};      // sums of 0 * o
+      const auto odd = [&] {
+        const float2 z = unpair(add2(add2(zero[0], zero[1]), add2(zero[2], zero[3])));
+        return !real ? 0 : top == INFINITY ? 2 : sees && sum < INFINITY && !(z.x + z.y == 0.f) ? 1 : 0;
+      };
       if (it.pieces > 1) {
         const int64_t at = (static_cast<int64_t>(it.slot) * p.kv_heads + it.kv) * 2 * kRows + t * kRows + row;
         if (real) p.part_ml[at] = make_float2(top, sum);
@@ -714,10 +738,12 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
           ptx::tmem_ld_32x32b_x32(col_o + 32 * c, o);
           ptx::tmem_ld_wait();
 #pragma unroll
+          for (int i = 0; i < 16; ++i) zero[i & 3] = fma2(pair(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), pair(0.f, 0.f), zero[i & 3]);
+#pragma unroll
           for (int i = 0; i < 4; ++i)
             if (real) write(reinterpret_cast<uint8_t*>(p.part_o + at * D), o + 8 * i, c * 128 + 32 * i, D * 4);
         }
-        return;
+        return odd();
       }
       // rows of one query are neighbours; the next query is all heads further
       uint8_t* to_row = reinterpret_cast<uint8_t*>(
@@ -729,14 +755,19 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         if (any) {
           ptx::tmem_ld_32x32b_x32(col_o + 32 * c, o);
           ptx::tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) zero[i & 3] = fma2(pair(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), pair(0.f, 0.f), zero[i & 3]);
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          v[i] = sees ? pack16<T>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv) : 0u;
+        for (int i = 0; i < 16; ++i) {
+          const float2 r = unpair(mul2(pair(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), pair(inv, inv)));
+          v[i] = sees ? pack16<T>(r.x, r.y) : 0u;
+        }
 #pragma unroll
         for (int i = 0; i < 2; ++i)
           if (real) write(to_row, v + 8 * i, c * 64 + 32 * i, p.dim * 2);
       }
+      return odd();
     };
     uint32_t x[kRows], e16[kRows / 2];
     uint64_t part[2];
@@ -863,8 +894,8 @@ attn_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
           o_phase ^= 1u;
           ptx::tc_fence_after_sync();
         }
-        output(items[done], done_any, done_sees, done_top, done_sum);
-        if (__any_sync(~0u, done_any && done_top == INFINITY)) row_by_row<T, D>(p, items[done], t, row);
+        const int odd = output(items[done], done_any, done_sees, done_top, done_sum);
+        if (__any_sync(~0u, odd)) row_by_row<T, D>(p, items[done], t, row, odd);
         __syncwarp();      // all lanes have read the item: its place is free
         if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(read_bar + done));
       }
