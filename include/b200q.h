@@ -472,8 +472,8 @@ int b200q_w8a8_gemm_noalloc(const int8_t* xq, const float* a_scales, const int8_
  * second product, and the result once.
  *
  * 16-bit elements [page][token][head][dim] at data + page * page_stride + token * token_stride + head *
- * head_stride (strides in elements, multiples of 8, not negative, under 2^39; the innermost dimension is dense, data
- * 16-byte aligned).
+ * head_stride (strides in elements, multiples of 8, not negative, under 2^39; the innermost dimension is dense,
+ * data 16-byte aligned).
  */
 typedef struct {
   void* data;
@@ -493,7 +493,7 @@ typedef struct {
   int tokens, key_tokens, sequences;
   int heads, kv_heads, dim;           /* dim % 8 == 0, dim <= 128; heads / kv_heads <= 128            */
   int pages, page_size, table_width;  /* page_size 0: packed, else a multiple of 16                   */
-  int max_q, max_k;                   /* bounds of n and m; results do not depend on them              */
+  int max_q, max_k;                   /* bounds of n (not used) and m (helps to divide the work)       */
   int causal;
   int dtype;                          /* B200Q_DTYPE_*                                                 */
   float scale;                        /* positive, under 1e38 */
@@ -503,8 +503,9 @@ typedef struct {
  * Sequences of any lengths, packed one after another (n = 0 and m = 0 included).  Decode: one query
  * per sequence, token b belongs to sequence b, keys and values in pages.  The lengths, tables and
  * pages are read on the device when the kernel runs, so a captured call follows their contents.
- * Lengths are cut to what the tables (packed: key_tokens, tokens) hold.  A page outside of the cache counts as zeros and
- * sets the device status word to 0xa01; cu_q that does not rise may set it to 0xa03 (and leaves rows unwritten).  workspace: *_workspace_bytes() of the same arguments (0 -> NULL ok);
+ * Lengths are cut to what the tables (packed: key_tokens, tokens) hold.  A page outside of the cache counts as
+ * zeros and sets the device status word to 0xa01; cu_q that does not rise may set it to 0xa03 (and leaves rows
+ * unwritten).  workspace: *_workspace_bytes() of the same arguments (0 -> NULL ok);
  * it holds nothing from one call to the next, and calls that overlap need one each.
  */
 int b200q_attn_prefill(const b200q_attention* a, void* workspace, size_t workspace_bytes, void* stream);
@@ -525,7 +526,8 @@ int b200q_kv_store(const b200q_view* k, const b200q_view* v, const b200q_view* k
 /*
  * Copies whole pages: page src[i] to page dst[i], in each of `outer` caches (layers, keys and values) that
  * begin outer_stride bytes apart and whose dense pages of page_bytes begin page_stride bytes apart (all
- * multiples of 16; pages do not overlap).  src and dst are HOST arrays, read before the call returns (a captured call keeps its pairs).
+ * multiples of 16; pages do not overlap).  src and dst are HOST arrays, read before the call returns (a captured
+ * call keeps its pairs).
  * A page may be copied to several places; a destination stands once, and no page is source and destination
  * of one call (B200Q_ERR_BAD_ARGUMENT, as for a page outside of the cache).  No counterpart in the reference.
  */

@@ -10,11 +10,12 @@ With ``G = heads / kv_heads`` and a sequence of ``n`` queries and ``m`` keys, th
 
     o[i, h] = sum_j p[i, h, j] v[j, h // G],    p = softmax_j(scale * q[i, h] . k[j, h // G])
 
-over ``j <= i + m - n`` (``causal``) or all ``j < m``; zeros where that leaves no key, or only scores of -infinity.  Sums and softmax statistics
-are fp32; the softmax weights are rounded to the tensors' type for the second product, as is the result.  What
-keys and values hold that a row does not see does not matter, NaN and infinities included.  Scores ``scale * q . k`` are
-fp32 and may be of any size up to 2^127.  Two things that no healthy model has make prompts slow, a hundred times for the rows
-concerned: scores beyond 700,000, and values that are not finite up to 255 positions behind a row that does not see them.
+over ``j <= i + m - n`` (``causal``) or all ``j < m``; zeros where that leaves no key, or only scores of -infinity.
+Sums and softmax statistics are fp32; the softmax weights are rounded to the tensors' type for the second product, as
+is the result.  What keys and values hold that a row does not see does not matter, NaN and infinities included.  Scores
+``scale * q . k`` are fp32 and may be of any size up to 2^127.  Two things that no healthy model has make prompts slow,
+a hundred times for the rows concerned: scores beyond 700,000, and values that are not finite up to 255 positions
+behind a row that does not see them.
 
 ``float16`` or ``bfloat16``; ``dim`` a multiple of 8 up to 128; up to 128 query heads per key head; pages of a
 multiple of 16 positions.  Heads, tokens and pages may stand apart (strides of a multiple of 8 elements).  Calls run on
@@ -115,12 +116,13 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seql
     packed by ``cu_seqlens_k``.  With ``block_tables`` (int32 ``[sequences, pages of the longest]``) they are a layer's
     caches ``[pages, page size, kv heads, dim]``, and position ``j`` of sequence ``b`` stands in page
     ``block_tables[b, j // page size]`` (a prompt whose beginning is cached, a chunk of a long one); of
-    ``cu_seqlens_k`` only the differences count.  Both ``cu_seqlens`` are int32 ``[sequences + 1]`` on the GPU;
-    ``max_seqlen_q`` and ``max_seqlen_k`` bound the lengths and only help to divide the work: the result does not
-    depend on them beyond rounding.  ``scale`` is positive and defaults to ``dim ** -0.5``.
+    ``cu_seqlens_k`` only the differences count.  Both ``cu_seqlens`` are int32 ``[sequences + 1]`` on the GPU.
+    ``max_seqlen_k`` bounds the keys of a sequence and only helps to divide the work: the result does not depend on it
+    beyond rounding.  ``max_seqlen_q`` belongs to the call as engines make it and is not used.  ``scale`` is positive
+    and defaults to ``dim ** -0.5``.
 
-    Returns ``[tokens, heads, dim]`` (``out``, where that is given, contiguous).  Rows behind the last sequence are
-    not written.
+    Returns ``[tokens, heads, dim]`` (``out``, where that is given, contiguous; it may be the memory of ``q``).  Rows
+    behind the last sequence are not written.
     """
     if scale is None:
         scale = max(q.shape[-1], 1) ** -0.5
